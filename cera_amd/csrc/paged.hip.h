@@ -1,0 +1,52 @@
+// Device-side view of a paged cache (cera_hip_paged_kv), shared by its kernels.
+#pragma once
+#include "common.hip.h"
+#include "host_common.h"
+#include "paged_plan.h"
+
+struct PagedView {
+    const int32_t* table;
+    const uint32_t* lens;
+    uint64_t page_stride, head_stride;   // elements
+    uint32_t n_kv, n_pages, max_pages, page_log2, max_len;
+};
+static inline PagedView paged_view(const cera_hip_paged_kv& c, uint32_t max_len) {
+    PagedView v{};
+    v.table = c.table;
+    v.lens = c.lens;
+    v.page_stride = paged_stride(c);
+    v.head_stride = static_cast<uint64_t>(c.page_size) * c.head_dim;
+    v.n_kv = c.n_kv_heads;
+    v.n_pages = c.n_pages;
+    v.max_pages = c.max_pages;
+    v.page_log2 = static_cast<uint32_t>(__builtin_ctz(c.page_size));
+    v.max_len = paged_max_len(c, max_len);
+    return v;
+}
+
+// The page of position t (t < max_len, so the table has its column); *ok turns false where the table names none of the pool's, and the
+// page is then 0, whose memory is there.
+__device__ __forceinline__ uint32_t paged_page(const PagedView& v, uint32_t seq, uint32_t t, bool& ok) {
+    const uint32_t p = static_cast<uint32_t>(v.table[static_cast<uint64_t>(seq) * v.max_pages + (t >> v.page_log2)]);
+    if (p >= v.n_pages) ok = false;
+    return p < v.n_pages ? p : 0u;
+}
+// element of position t's row of kv head g
+template <int HD>
+__device__ __forceinline__ uint64_t paged_row(const PagedView& v, uint32_t page, uint32_t g, uint32_t t) {
+    return page * v.page_stride + g * v.head_stride + static_cast<uint64_t>(t & ((1u << v.page_log2) - 1)) * HD;
+}
+
+// The context's device while a call lasts: a caller may have made another one current.
+struct PagedDevice {
+    int before = -1;
+    hipError_t err = hipSuccess;
+    explicit PagedDevice(int device) {
+        if ((err = hipGetDevice(&before)) != hipSuccess) { before = -1; return; }
+        if (before == device) before = -1;
+        else err = hipSetDevice(device);
+    }
+    ~PagedDevice() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};

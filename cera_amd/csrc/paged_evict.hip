@@ -1,0 +1,169 @@
+// Eviction from a paged cache by accumulated attention weight (cera_hip_paged_evict_dev; contract in include/cera_hip.h).
+//
+// Two launches.  The first chooses: a workgroup per (kv head, sequence) finds the weight of the last position that stays by radix
+// selection on the weights' bits, in three passes of 11, 11 and 10 bits, and writes the positions that stay in their order.  The
+// second moves: position i takes the row of position kept[i] >= i, so that a walk upwards in place never reads what it has
+// written, as long as all rows of a step are read before the step writes.
+#include "paged.hip.h"
+
+static constexpr uint32_t EV_THREADS = 1024, EV_BINS = 2048;
+
+// a weight as an integer of the same order: -0 as 0, every NaN above all numbers
+__device__ __forceinline__ uint32_t evict_key(float w) {
+    if (w != w) return 0xFFFFFFFFu;
+    const uint32_t b = __builtin_bit_cast(uint32_t, w + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// grid = (kv heads, sequences).  kept: [n_seqs][n_kv][budget]; cut[s]: positions of a sequence that is cut, else 0
+__global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedView c, float* __restrict__ mass, uint64_t mass_stride, uint32_t budget, uint32_t n_first,
+                                                                        uint32_t n_recent, uint32_t* __restrict__ kept_ws, int32_t* __restrict__ kept_out,
+                                                                        uint32_t* __restrict__ new_lens, uint32_t* __restrict__ cut) {
+    __shared__ uint32_t hist[EV_BINS], wave_tot[EV_THREADS / 64], sh[4];
+    const uint32_t g = blockIdx.x, s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t len = c.lens[s];
+    const uint64_t sg = static_cast<uint64_t>(s) * c.n_kv + g;
+    bool ok = len <= c.max_len;
+    if (ok)
+        for (uint32_t p = tid; p << c.page_log2 < len; p += EV_THREADS) (void)paged_page(c, s, p << c.page_log2, ok);
+    ok = __syncthreads_and(ok);
+    int32_t* const out = kept_out ? kept_out + sg * budget : nullptr;
+    if (!ok || len <= budget) {
+        if (out)
+            for (uint32_t i = tid; i < budget; i += EV_THREADS) out[i] = ok && i < len ? static_cast<int32_t>(i) : -1;
+        if (g == 0 && tid == 0) { new_lens[s] = len; cut[s] = 0; }
+        return;
+    }
+    float* const mw = mass + sg * mass_stride;
+    // the middle [lo, hi) has more than `need` positions
+    const uint32_t lo = n_first, hi = len - n_recent, need = budget - n_first - n_recent;
+    // radix selection: `prefix` holds the bits found so far, `left` how many of those that share them still stay
+    uint32_t prefix = 0, left = need;
+    if (need) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, above = shift + bits;
+            for (uint32_t b = tid; b < EV_BINS; b += EV_THREADS) hist[b] = 0;
+            __syncthreads();
+            for (uint32_t t = lo + tid; t < hi; t += EV_THREADS) {
+                const uint32_t k = evict_key(mw[t]);
+                if (pass == 0 || k >> above == prefix >> above) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
+            }
+            __syncthreads();
+            // from the top bin down to the one in which the count reaches `left`: two bins a thread, thread 0 has the highest
+            const uint32_t top = (1u << bits) - 1, n_thr = (1u << bits) / 2;
+            uint32_t a = 0, b = 0;
+            if (tid < n_thr) { a = hist[top - 2 * tid]; b = hist[top - 2 * tid - 1]; }
+            uint32_t sum = a + b, inc = sum;
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = __shfl_up(inc, d);
+                if (lane >= static_cast<uint32_t>(d)) inc += o;
+            }
+            if (lane == 63) wave_tot[w] = inc;
+            __syncthreads();
+            uint32_t before = inc - sum;
+            for (uint32_t i = 0; i < w; ++i) before += wave_tot[i];
+            if (before < left && before + sum >= left) {
+                const bool second = before + a < left;
+                sh[0] = prefix | (top - 2 * tid - (second ? 1 : 0)) << shift;
+                sh[1] = left - before - (second ? a : 0);
+            }
+            __syncthreads();
+            prefix = sh[0];
+            left = sh[1];
+        }
+    }
+    // in order: larger ones and the ends stay, of the equal ones the first `left`
+    uint32_t base_gt = 0, base_eq = 0;
+    uint32_t* const ws = kept_ws + sg * budget;
+    for (uint32_t t0 = 0; t0 < len; t0 += EV_THREADS) {
+        const uint32_t t = t0 + tid;
+        const bool in = t < len, mid = in && t >= lo && t < hi;
+        const float x = in ? mw[t] : 0.0f;
+        const uint32_t k = evict_key(x);
+        const bool gt = in && (!mid || (need && k > prefix)), eq = mid && need && k == prefix;
+        const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
+        if (lane == 0) wave_tot[w] = __popcll(bg) | __popcll(be) << 16;
+        __syncthreads();
+        uint32_t sg_ = 0, se_ = 0, tg = 0, te = 0;
+        for (uint32_t i = 0; i < EV_THREADS / 64; ++i) {
+            const uint32_t v = wave_tot[i];
+            if (i < w) { sg_ += v & 0xFFFF; se_ += v >> 16; }
+            tg += v & 0xFFFF;
+            te += v >> 16;
+        }
+        const uint32_t n_gt = base_gt + sg_ + __popcll(bg & below), n_eq = base_eq + se_ + __popcll(be & below);
+        if (gt || (eq && n_eq < left)) {
+            const uint32_t dst = n_gt + min(n_eq, left);
+            ws[dst] = t;
+            if (out) out[dst] = static_cast<int32_t>(t);
+            mw[dst] = x;   // dst <= t, and all of this step's weights are read
+        }
+        base_gt += tg;
+        base_eq += te;
+        __syncthreads();
+    }
+    if (g == 0 && tid == 0) { new_lens[s] = budget; cut[s] = len; }
+}
+
+// grid = (128-byte columns of a row, 2 * kv heads, sequences): keys, then values.  Eight lanes of 16 bytes a row.
+static constexpr uint32_t EV_ROWS = 32, EV_UNROLL = 8;   // rows of a workgroup's pass, passes of a step
+template <typename KV, int HD>
+__global__ __launch_bounds__(256) void paged_evict_move_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, uint32_t budget, const uint32_t* __restrict__ kept,
+                                                               const uint32_t* __restrict__ cut) {
+    const uint32_t s = blockIdx.z, g = blockIdx.y >> 1, j = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+    if (cut[s] == 0) return;
+    KV* const pool = blockIdx.y & 1 ? vp : kp;
+    const uint32_t col = (blockIdx.x * 128 + j * 16) / sizeof(KV);
+    const uint32_t* const idx = kept + (static_cast<uint64_t>(s) * c.n_kv + g) * budget;
+    constexpr uint32_t STEP = EV_ROWS * EV_UNROLL;
+    uint4 row[EV_UNROLL];
+    bool ok = true;   // the pages were looked over when the positions were chosen
+    for (uint32_t i0 = 0; i0 < budget; i0 += STEP) {
+        for (uint32_t u = 0; u < EV_UNROLL; ++u) {
+            const uint32_t i = i0 + u * EV_ROWS + r0;
+            if (i < budget) {
+                const uint32_t t = idx[i];
+                row[u] = *reinterpret_cast<const uint4*>(pool + paged_row<HD>(c, paged_page(c, s, t, ok), g, t) + col);
+            }
+        }
+        __syncthreads();   // every row of the step is read
+        for (uint32_t u = 0; u < EV_UNROLL; ++u) {
+            const uint32_t i = i0 + u * EV_ROWS + r0;
+            if (i < budget) *reinterpret_cast<uint4*>(pool + paged_row<HD>(c, paged_page(c, s, i, ok), g, i) + col) = row[u];
+        }
+    }
+}
+
+template <typename KV, int HD>
+static void paged_evict_launch(cera_hip_ctx* ctx, const cera_hip_paged_kv& c, const cera_hip_paged_evict& e, uint32_t* kept, uint32_t* cut) {
+    const PagedView v = paged_view(c, e.max_len);
+    hipLaunchKernelGGL(paged_evict_select_kernel, dim3(c.n_kv_heads, c.n_seqs), dim3(EV_THREADS), 0, ctx->stream, v, e.mass, e.mass_stride, e.budget, e.n_first, e.n_recent, kept, e.kept,
+                       e.new_lens, cut);
+    hipLaunchKernelGGL((paged_evict_move_kernel<KV, HD>), dim3(HD * sizeof(KV) / 128, 2 * c.n_kv_heads, c.n_seqs), dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v),
+                       e.budget, kept, cut);
+}
+
+extern "C" cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx* ctx, const cera_hip_paged_kv* c, const cera_hip_paged_evict* e) {
+    if (!ctx) return CERA_HIP_ERR_ARGUMENT;
+    std::lock_guard<std::recursive_mutex> op_lk(ctx->op_mu);
+    const PagedCheck no = paged_check_evict(c, e);
+    if (no.msg) return cera_fail(ctx, no.st, no.msg);
+    if (c->n_seqs == 0) return CERA_HIP_OK;
+    const PagedDevice dev(ctx->device);
+    HIP_TRY(ctx, dev.err);
+    // a budget behind the longest sequence cuts none; the list then needs no room
+    const uint64_t list = e->budget < paged_max_len(*c, e->max_len) ? static_cast<uint64_t>(c->n_seqs) * c->n_kv_heads * e->budget : 0;
+    void* ws;
+    CERA_TRY(cera_scratch(ctx, 15, (list + c->n_seqs) * 4, &ws));
+    uint32_t* const cut = static_cast<uint32_t*>(ws);
+    uint32_t* const kept = cut + c->n_seqs;
+    if (c->kv_type == CERA_HIP_KV_F16) {
+        if (c->head_dim == 128) paged_evict_launch<kv_half, 128>(ctx, *c, *e, kept, cut);
+        else paged_evict_launch<kv_half, 64>(ctx, *c, *e, kept, cut);
+    } else {
+        if (c->head_dim == 128) paged_evict_launch<float, 128>(ctx, *c, *e, kept, cut);
+        else paged_evict_launch<float, 64>(ctx, *c, *e, kept, cut);
+    }
+    HIP_TRY(ctx, hipGetLastError());
+    return CERA_HIP_OK;
+}

@@ -1,0 +1,124 @@
+// What the calls on a paged cache check on the host, and which positions a row sees.  Plain arithmetic, without the device's headers.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "cera_hip.h"
+
+#if defined(__HIPCC__)
+#define PAGED_HD __host__ __device__ inline
+#else
+#define PAGED_HD inline
+#endif
+
+struct PagedCheck {
+    cera_hip_status st;
+    const char* msg;   // null: in order
+};
+inline PagedCheck paged_no(cera_hip_status st, const char* msg) { return {st, msg}; }
+inline bool paged_aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+inline uint64_t paged_capacity(const cera_hip_paged_kv& c) { return static_cast<uint64_t>(c.max_pages) * c.page_size; }
+inline uint64_t paged_stride(const cera_hip_paged_kv& c) {
+    return c.page_stride ? c.page_stride : static_cast<uint64_t>(c.n_kv_heads) * c.page_size * c.head_dim;
+}
+// the longest sequence that a call may meet
+inline uint32_t paged_max_len(const cera_hip_paged_kv& c, uint32_t max_len) {
+    const uint64_t cap = paged_capacity(c);
+    return static_cast<uint32_t>(max_len ? std::min<uint64_t>(max_len, cap) : cap);
+}
+
+inline PagedCheck paged_check_kv(const cera_hip_paged_kv* c) {
+    if (!c) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged cache: null");
+    if (c->kv_type != CERA_HIP_KV_F32 && c->kv_type != CERA_HIP_KV_F16) return paged_no(CERA_HIP_ERR_UNSUPPORTED_DTYPE, "paged cache: kv_type is CERA_HIP_KV_F32 or CERA_HIP_KV_F16");
+    if (!c->k || !c->v || !c->table || !c->lens) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged cache: k, v, table or lens is null");
+    if (c->head_dim != 64 && c->head_dim != 128) return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: head_dim 64 or 128");
+    if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: page_size 16, 32, 64, 128 or 256");
+    if (c->n_kv_heads == 0 || c->n_kv_heads > 1024) return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: 1 to 1024 kv heads");
+    if (c->n_pages == 0 || c->n_pages > 0x7FFFFFFFu || c->max_pages == 0 || paged_capacity(*c) > (1ull << 30)) return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: pages of the pool, pages of a sequence (at most 2^30 positions)");
+    if (c->n_seqs > 65535) return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: at most 65535 sequences");
+    if (c->page_stride && (c->page_stride % 8 || c->page_stride < static_cast<uint64_t>(c->n_kv_heads) * c->page_size * c->head_dim || c->page_stride > (1ull << 40)))
+        return paged_no(CERA_HIP_ERR_SHAPE, "paged cache: page_stride is below a page, or no multiple of 8");
+    if (!paged_aligned(c->k, 16) || !paged_aligned(c->v, 16) || !paged_aligned(c->table, 4) || !paged_aligned(c->lens, 4)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged cache: k and v are 16-byte aligned, table and lens 4-byte");
+    return {CERA_HIP_OK, nullptr};
+}
+
+inline bool paged_row_stride_ok(uint64_t stride, uint64_t row) { return stride == 0 || (stride >= row && stride % 4 == 0 && stride <= (1ull << 40)); }
+
+inline PagedCheck paged_check_attn(const cera_hip_paged_kv* c, const cera_hip_paged_attn* a) {
+    const PagedCheck kv = paged_check_kv(c);
+    if (kv.msg) return kv;
+    if (!a || !a->q || !a->out) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: q or out is null");
+    if (!a->k_new != !a->v_new) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: k_new and v_new come together");
+    if (a->n_heads == 0 || a->n_heads % c->n_kv_heads || a->n_heads > 65536) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: n_heads must be a multiple of n_kv_heads");
+    if (!std::isfinite(a->scale)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: scale must be finite");
+    if (!a->q_first && a->n_rows != c->n_seqs) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: without q_first there is one row a sequence");
+    if (a->n_rows > (1u << 30)) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: at most 2^30 rows");
+    const uint64_t q_row = static_cast<uint64_t>(a->n_heads) * c->head_dim, kv_row = static_cast<uint64_t>(c->n_kv_heads) * c->head_dim;
+    if (!paged_row_stride_ok(a->q_stride, q_row) || !paged_row_stride_ok(a->out_stride, q_row) || !paged_row_stride_ok(a->kv_stride, kv_row))
+        return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: a stride is below a row, or no multiple of 4");
+    if (!paged_aligned(a->q, 16) || !paged_aligned(a->out, 16) || !paged_aligned(a->k_new, 16) || !paged_aligned(a->v_new, 16) || !paged_aligned(a->q_first, 4) || !paged_aligned(a->mass, 4))
+        return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: q, k_new, v_new and out are 16-byte aligned, q_first and mass 4-byte");
+    if (a->mass && a->q_first) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: mass goes with one row a sequence");
+    if (a->mass && (a->mass_stride < paged_max_len(*c, a->max_len) || a->mass_stride > (1ull << 40))) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: mass_stride is below the longest sequence");
+    return {CERA_HIP_OK, nullptr};
+}
+
+inline PagedCheck paged_check_evict(const cera_hip_paged_kv* c, const cera_hip_paged_evict* e) {
+    const PagedCheck kv = paged_check_kv(c);
+    if (kv.msg) return kv;
+    if (!e || !e->mass || !e->new_lens) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged eviction: mass or new_lens is null");
+    if (e->new_lens == c->lens) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged eviction: new_lens is not lens");
+    if (!paged_aligned(e->mass, 4) || !paged_aligned(e->new_lens, 4) || !paged_aligned(e->kept, 4)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged eviction: mass, new_lens and kept are 4-byte aligned");
+    if (e->budget == 0 || e->budget > (1u << 30) || static_cast<uint64_t>(e->n_first) + e->n_recent > e->budget) return paged_no(CERA_HIP_ERR_SHAPE, "paged eviction: n_first + n_recent <= budget, budget from 1");
+    if (e->mass_stride < paged_max_len(*c, e->max_len) || e->mass_stride > (1ull << 40)) return paged_no(CERA_HIP_ERR_SHAPE, "paged eviction: mass_stride is below the longest sequence");
+    return {CERA_HIP_OK, nullptr};
+}
+
+inline PagedCheck verify_check(const cera_hip_verify_draft* d) {
+    if (!d || !d->target || !d->tokens || !d->uniform || !d->accepted || !d->out_tokens) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: a pointer is null");
+    if (d->vocab == 0 || d->vocab > (1u << 24)) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: a vocabulary of 1 to 2^24 tokens");
+    if (d->max_draft == 0 || d->max_draft > 64) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: 1 to 64 drafted tokens");
+    if (d->n_seqs > 65535) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: at most 65535 sequences");
+    if (!(d->temperature >= 0) || !std::isfinite(d->temperature)) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: temperature is finite, 0 or more");
+    if (d->row_stride && (d->row_stride < d->vocab || d->row_stride > (1ull << 40))) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: row_stride is below the vocabulary");
+    for (const void* p : {static_cast<const void*>(d->target), static_cast<const void*>(d->draft), static_cast<const void*>(d->tokens), static_cast<const void*>(d->n_draft),
+                          static_cast<const void*>(d->uniform), static_cast<const void*>(d->accepted), static_cast<const void*>(d->out_tokens)})
+        if (!paged_aligned(p, 4)) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: pointers are 4-byte aligned");
+    return {CERA_HIP_OK, nullptr};
+}
+
+// The rows of one sequence in a call.
+struct PagedRows {
+    uint32_t first, n;   // rows of q and out; n = 0: none
+    uint32_t len;        // positions of the sequence; row first + i is at position len - n + i
+    bool bad;            // lengths or rows out of order: [first, first + n) get NaN, nothing else is touched
+};
+PAGED_HD PagedRows paged_rows(const uint32_t* q_first, const uint32_t* lens, uint32_t s, uint32_t n_rows, uint32_t max_queries, uint32_t max_len) {
+    PagedRows r;
+    r.len = lens[s];
+    if (!q_first) {
+        r.first = s;
+        r.n = 1;
+        r.bad = r.len > max_len;
+        return r;
+    }
+    const uint32_t a = q_first[s], b = q_first[s + 1];
+    r.bad = a > b || b > n_rows || b - a > max_queries || b - a > r.len || r.len > max_len;
+    r.first = a < n_rows ? a : n_rows;
+    const uint32_t end = b < n_rows ? b : n_rows;
+    r.n = end > r.first ? end - r.first : 0;
+    return r;
+}
+
+// Positions that the row at position P sees: [0, sink_end) and [start, P], sink_end <= start.
+struct PagedSeen {
+    uint32_t sink_end, start;
+};
+PAGED_HD PagedSeen paged_seen(uint32_t P, uint32_t window, uint32_t n_sink) {
+    PagedSeen v;
+    v.start = window && P + 1 > window ? P + 1 - window : 0;
+    v.sink_end = n_sink < v.start ? n_sink : v.start;
+    return v;
+}

@@ -36,6 +36,7 @@ SYMBOLS = [
     "cera_hip_rmsnorm_q8_0", "cera_hip_attn_decode_step", "cera_hip_attn_decode_dev_noalloc", "cera_hip_gemm_block_dots",
     "cera_hip_ffn_gate_up_fused", "cera_hip_qkv_fused",
     "cera_hip_layered_create", "cera_hip_dense_tile", "cera_hip_dense_streams_tile", "cera_hip_read_conv", "cera_hip_write_conv",
+    "cera_hip_paged_attn_dev", "cera_hip_paged_evict_dev", "cera_hip_verify_draft_dev",
 ]
 
 
@@ -104,6 +105,32 @@ class DecodeOp(C.Structure):
     _fields_ = [("kind", C.c_uint32), ("n", C.c_uint32), ("w", C.c_void_p), ("w2", C.c_void_p), ("x", C.c_void_p),
                 ("norm_w", C.c_void_p), ("eps", C.c_float), ("xs", C.c_void_p), ("xq", C.c_void_p), ("resid", C.c_void_p),
                 ("y", C.c_void_p), ("y2", C.c_void_p), ("out_s", C.c_void_p), ("out_q", C.c_void_p)]
+
+
+class PagedKV(C.Structure):
+    """cera_hip_paged_kv: a pool of cache pages, the sequences' table and lengths (device pointers)."""
+    _fields_ = [(n, C.c_uint32) for n in ("kv_type", "n_kv_heads", "head_dim", "page_size", "n_pages", "n_seqs", "max_pages", "_reserved")] + \
+               [("page_stride", C.c_uint64)] + [(n, C.c_void_p) for n in ("k", "v", "table", "lens")]
+
+
+class PagedAttn(C.Structure):
+    """cera_hip_paged_attn."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_new", "v_new", "out", "mass", "q_first")] + \
+               [(n, C.c_uint64) for n in ("q_stride", "kv_stride", "out_stride", "mass_stride")] + \
+               [(n, C.c_uint32) for n in ("n_rows", "max_queries", "n_heads")] + [("scale", C.c_float)] + \
+               [(n, C.c_uint32) for n in ("window", "n_sink", "max_len", "_reserved")]
+
+
+class PagedEvict(C.Structure):
+    """cera_hip_paged_evict."""
+    _fields_ = [("mass", C.c_void_p), ("mass_stride", C.c_uint64), ("new_lens", C.c_void_p), ("kept", C.c_void_p)] + \
+               [(n, C.c_uint32) for n in ("budget", "n_first", "n_recent", "max_len")]
+
+
+class VerifyDraft(C.Structure):
+    """cera_hip_verify_draft."""
+    _fields_ = [(n, C.c_uint32) for n in ("n_seqs", "max_draft", "vocab")] + [("temperature", C.c_float), ("row_stride", C.c_uint64)] + \
+               [(n, C.c_void_p) for n in ("target", "draft", "tokens", "n_draft", "uniform", "accepted", "out_tokens")]
 
 
 _lib = None
@@ -191,6 +218,9 @@ def load_library() -> C.CDLL:
         "cera_hip_dense_streams_tile": (u32, [u64, u64, u32, u32, u64, u32, C.POINTER(u32)]),
         "cera_hip_read_conv": (i32, [vp, u32, vp]), "cera_hip_write_conv": (i32, [vp, u32, vp, u32]),
         "cera_hip_rmsnorm_q8_0": (i32, [vp, vp, vp, u64, f32, vp, vp, vp]),
+        "cera_hip_paged_attn_dev": (i32, [vp, C.POINTER(PagedKV), C.POINTER(PagedAttn)]),
+        "cera_hip_paged_evict_dev": (i32, [vp, C.POINTER(PagedKV), C.POINTER(PagedEvict)]),
+        "cera_hip_verify_draft_dev": (i32, [vp, C.POINTER(VerifyDraft)]),
         "cera_hip_attn_decode_step": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, f32, u32, vp, f32, u32,
                                             vp, vp, vp, vp, vp]),
     }
@@ -504,6 +534,19 @@ class Context:
         self.check(self.lib.cera_hip_qkv_fused(self.h, C.byref(ta), C.byref(tb) if tb is not None else None, _p(x), _p(nw), eps,
                                                _p(ya), _p(yb) if yb is not None else None))
         return ya, yb
+
+    # -- many sequences in one pool of cache pages, device buffers
+    def paged_attn(self, cache: PagedKV, op: PagedAttn):
+        """Writes the new tokens' keys and values into their pages, if there are any, and attends; queues only."""
+        self.check(self.lib.cera_hip_paged_attn_dev(self.h, cache, op))
+
+    def paged_evict(self, cache: PagedKV, op: PagedEvict):
+        """Brings every sequence back to a budget of positions, by accumulated attention weight; queues only."""
+        self.check(self.lib.cera_hip_paged_evict_dev(self.h, cache, op))
+
+    def verify_draft(self, op: VerifyDraft):
+        """Decides about drafted tokens and draws the next one; queues only."""
+        self.check(self.lib.cera_hip_verify_draft_dev(self.h, op))
 
     # -- the decode step's fused kernels
     def rmsnorm_q8_0(self, x, w, eps):

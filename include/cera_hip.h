@@ -467,6 +467,117 @@ CERA_HIP_API cera_hip_status cera_hip_attn_decode_f16_dev(cera_hip_ctx*, const f
 CERA_HIP_API cera_hip_status cera_hip_gemm_dev(cera_hip_ctx*, const cera_hip_dtensor* w, const float* x, uint64_t n,
                                                float* out);
 
+/* ---- many sequences in one pool of cache pages, device buffers ------------ */
+/* The cache of a server: a pool of pages that any number of sequences share out among themselves.
+ * Every pointer is a device pointer on the context's device and the calls only queue work on the
+ * context's stream; the host checks what it can see (CERA_HIP_ERR_SHAPE / _ARGUMENT /
+ * _UNSUPPORTED_DTYPE), the kernels check what lies on the device -- page numbers, lengths, row
+ * ranges -- before they use it, and never touch memory outside the pool.  No counterpart in the
+ * reference, which has one sequence per cache (cera/src/kv_cache.rs:201-221).
+ *
+ * k and v hold pages [n_kv_heads][page_size][head_dim] of f32 or IEEE half (kv_type), page p at
+ * element p * page_stride (0: one behind the other), both 16-byte aligned; keys are stored rotated.
+ * Position t of sequence s is slot t % page_size of page table[s * max_pages + t / page_size].
+ * Entries whose positions a call does not use are not read as page numbers and may hold anything.
+ * Pages may be shared between sequences as long as no call writes to them.  head_dim 64 or 128;
+ * page_size 16, 32, 64, 128 or 256; at most 65535 sequences and 2^30 positions in a row of the table. */
+typedef struct {
+    uint32_t kv_type;    /* CERA_HIP_KV_F32 or CERA_HIP_KV_F16 */
+    uint32_t n_kv_heads, head_dim, page_size;
+    uint32_t n_pages;    /* pages of the pool */
+    uint32_t n_seqs, max_pages; /* rows and columns of the table */
+    uint32_t _reserved;
+    uint64_t page_stride; /* elements, a multiple of 8; 0: n_kv_heads * page_size * head_dim */
+    void *k, *v;
+    const int32_t* table;  /* [n_seqs][max_pages] */
+    const uint32_t* lens;  /* [n_seqs] positions of each sequence, the call's own rows counted */
+} cera_hip_paged_kv;
+
+/* Attention of new tokens to their sequences (transformer::decode_attention, cera/src/model/
+ * transformer.rs:1249-1305, for a batch of sequences), with an optional sliding window.
+ * q_first null, the decode form: row s of q is sequence s's one new token, at position lens[s] - 1;
+ * n_rows = n_seqs.  Otherwise rows q_first[s] .. q_first[s + 1] are the last positions of sequence s,
+ * at most max_queries of them (0: n_rows); rows that belong to no sequence are left as they are.
+ * Row at position P sees positions t <= P with t < n_sink or window == 0 or t > P - window;
+ * out = sum_t softmax_t(scale * q . K[t]) V[t], zeros where it sees nothing (a sequence of length 0).
+ * k_new / v_new (both or neither): the rows' own keys and values, [n_rows][n_kv_heads * head_dim]
+ * f32, which are written into the pages first (narrowed to half to the nearest even) and so have to
+ * be in pages of their own sequence only.
+ * mass (nullable, decode form): mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
+ * g's query heads of the softmax weight of position t; with k_new, the new position's starts at 0.
+ * Memory: mass and many parts take a workspace of the context (about 4 bytes * n_heads * max_len per
+ * sequence for mass).  Results do not depend on other sequences of the call or on earlier calls.
+ * Host refusals: n_heads not a multiple of n_kv_heads, scale not finite, pointers not 16-byte (lens,
+ * table, q_first, mass: 4-byte) aligned, strides below a row or no multiple of 4 floats.
+ * On the device: a sequence with lens[s] > max_len (0: the table's capacity), a page number outside
+ * the pool among the positions it uses, or rows that decrease, end behind n_rows, outnumber
+ * max_queries or lens[s], gets NaN in its rows of out, and neither its pages nor its mass change
+ * unless all of its lengths and rows are in order (with a bad page, rows and weights that live
+ * in good pages may have been written). */
+typedef struct {
+    const float *q, *k_new, *v_new; /* rows of n_heads / n_kv_heads / n_kv_heads * head_dim floats */
+    float* out;
+    float* mass;
+    const uint32_t* q_first;                   /* nullable, [n_seqs + 1] */
+    uint64_t q_stride, kv_stride, out_stride;  /* floats between rows; 0: dense */
+    uint64_t mass_stride;                      /* floats between kv heads, at least max_len */
+    uint32_t n_rows, max_queries, n_heads;
+    float scale;
+    uint32_t window, n_sink;
+    uint32_t max_len, _reserved;
+} cera_hip_paged_attn;
+CERA_HIP_API cera_hip_status cera_hip_paged_attn_dev(cera_hip_ctx*, const cera_hip_paged_kv*, const cera_hip_paged_attn*);
+
+/* Brings every sequence back to `budget` positions, kv head by kv head: of a sequence with
+ * lens[s] > budget, the first n_first and the last n_recent positions stay, and between them the
+ * budget - n_first - n_recent with the largest mass, of equal ones the lowest (a NaN counts as
+ * larger than every number, -0 as 0).  What stays keeps its order and its rotation; keys, values and
+ * mass move down in place to positions 0 .. budget - 1.  new_lens[s] = min(lens[s], budget), which
+ * the caller uses as lens from then on (it may not be the array lens itself); kept (nullable,
+ * [n_seqs][n_kv_heads][budget]): the former position of each that stays, -1 behind the last.
+ * The positions' rank among the kv heads differs, so a cache that has been cut has no position
+ * numbers in common with its tokens: a window then counts kept positions.  Pages of the moved
+ * positions may not be shared.  n_first + n_recent <= budget, budget >= 1.
+ * A sequence with lens[s] > max_len or a bad page number among its pages is left as it is, with
+ * new_lens[s] = lens[s] and kept all -1.  What `shift_kv` does for a run of positions
+ * (cera/src/kv_cache.rs:1091-1310) without a choice by weight. */
+typedef struct {
+    float* mass;
+    uint64_t mass_stride;
+    uint32_t* new_lens;
+    int32_t* kept;
+    uint32_t budget, n_first, n_recent, max_len;
+} cera_hip_paged_evict;
+CERA_HIP_API cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx*, const cera_hip_paged_kv*, const cera_hip_paged_evict*);
+
+/* Decides about drafted tokens and draws the next one, from given random numbers (verify_draft's
+ * step for sampled text, on the logits that a chunk of drafts gives, one more row than drafts:
+ * cera/src/model/mod.rs:221-249).  Per sequence, p_i = softmax(target[i] / temperature),
+ * q_i = softmax(draft[i] / temperature), or, with draft null (tokens looked up, not drawn), all of
+ * q_i on the drafted token.  Token i is accepted if all before it are and uniform[i] * q_i(token) <
+ * p_i(token).  The next token is drawn from max(p_j - q_j, 0) at the first rejected j (from p_j where
+ * that is nothing everywhere), from p_n behind n accepted drafts: the first token at which the
+ * running sum in the order of the vocabulary exceeds uniform[max_draft] times its total.  All in
+ * 64 bits; logits may be -inf (such a token is never drawn).  temperature 0: a token is accepted if it
+ * is the row's largest logit (the lowest index of equals), and the next token is that of row j;
+ * uniform and draft are not read.
+ * out_tokens[s] = accepted drafts, the next token, then -1.  A row with a NaN or +inf, or with nothing
+ * but -inf, ends its sequence with next token -1; so does n_draft[s] > max_draft, with none accepted.
+ * A drafted token outside the vocabulary is rejected, and takes nothing away from p. */
+typedef struct {
+    uint32_t n_seqs, max_draft, vocab;
+    float temperature;        /* 0 or more */
+    uint64_t row_stride;      /* floats between rows of target and draft; 0: vocab */
+    const float* target;      /* [n_seqs][max_draft + 1] rows */
+    const float* draft;       /* nullable, [n_seqs][max_draft] rows */
+    const int32_t* tokens;    /* [n_seqs][max_draft] */
+    const uint32_t* n_draft;  /* nullable (all max_draft), [n_seqs] */
+    const float* uniform;     /* [n_seqs][max_draft + 1] in [0, 1) */
+    uint32_t* accepted;       /* [n_seqs] */
+    int32_t* out_tokens;      /* [n_seqs][max_draft + 1] */
+} cera_hip_verify_draft;
+CERA_HIP_API cera_hip_status cera_hip_verify_draft_dev(cera_hip_ctx*, const cera_hip_verify_draft*);
+
 /* ---- model level: the `Model` trait surface ------------------------------ */
 
 /* load_model_gpu-style construction from resolved weights

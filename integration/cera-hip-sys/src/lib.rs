@@ -250,6 +250,81 @@ pub struct cera_hip_decode_op {
     pub out_q: *mut i8,
 }
 
+/// A pool of cache pages with the table and the lengths of the sequences in it (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct cera_hip_paged_kv {
+    pub kv_type: u32,
+    pub n_kv_heads: u32,
+    pub head_dim: u32,
+    pub page_size: u32,
+    pub n_pages: u32,
+    pub n_seqs: u32,
+    pub max_pages: u32,
+    pub _reserved: u32,
+    pub page_stride: u64,
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub table: *const i32,
+    pub lens: *const u32,
+}
+
+/// Attention of new tokens over a paged cache.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct cera_hip_paged_attn {
+    pub q: *const f32,
+    pub k_new: *const f32,
+    pub v_new: *const f32,
+    pub out: *mut f32,
+    pub mass: *mut f32,
+    pub q_first: *const u32,
+    pub q_stride: u64,
+    pub kv_stride: u64,
+    pub out_stride: u64,
+    pub mass_stride: u64,
+    pub n_rows: u32,
+    pub max_queries: u32,
+    pub n_heads: u32,
+    pub scale: f32,
+    pub window: u32,
+    pub n_sink: u32,
+    pub max_len: u32,
+    pub _reserved: u32,
+}
+
+/// Eviction from a paged cache by accumulated attention weight.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct cera_hip_paged_evict {
+    pub mass: *mut f32,
+    pub mass_stride: u64,
+    pub new_lens: *mut u32,
+    pub kept: *mut i32,
+    pub budget: u32,
+    pub n_first: u32,
+    pub n_recent: u32,
+    pub max_len: u32,
+}
+
+/// Verification of drafted tokens from given random numbers.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct cera_hip_verify_draft {
+    pub n_seqs: u32,
+    pub max_draft: u32,
+    pub vocab: u32,
+    pub temperature: f32,
+    pub row_stride: u64,
+    pub target: *const f32,
+    pub draft: *const f32,
+    pub tokens: *const i32,
+    pub n_draft: *const u32,
+    pub uniform: *const f32,
+    pub accepted: *mut u32,
+    pub out_tokens: *mut i32,
+}
+
 unsafe extern "C" {
 pub fn cera_hip_ctx_create(
         device: c_int,
@@ -658,6 +733,20 @@ pub fn cera_hip_ctx_create(
         n: u64,
         out: *mut f32,
     ) -> cera_hip_status;
+    pub fn cera_hip_paged_attn_dev(
+        ctx: *mut cera_hip_ctx,
+        cache: *const cera_hip_paged_kv,
+        op: *const cera_hip_paged_attn,
+    ) -> cera_hip_status;
+    pub fn cera_hip_paged_evict_dev(
+        ctx: *mut cera_hip_ctx,
+        cache: *const cera_hip_paged_kv,
+        op: *const cera_hip_paged_evict,
+    ) -> cera_hip_status;
+    pub fn cera_hip_verify_draft_dev(
+        ctx: *mut cera_hip_ctx,
+        op: *const cera_hip_verify_draft,
+    ) -> cera_hip_status;
     pub fn cera_hip_model_create(
         ctx: *mut cera_hip_ctx,
         config: *const cera_hip_config,
@@ -760,5 +849,9 @@ mod tests {
         assert_eq!(align_of::<cera_hip_config>(), 8);
         assert_eq!(size_of::<cera_hip_gemv_op>(), 40);
         assert_eq!(size_of::<cera_hip_decode_op>(), 104);
+        assert_eq!(size_of::<cera_hip_paged_kv>(), 72);
+        assert_eq!(size_of::<cera_hip_paged_attn>(), 112);
+        assert_eq!(size_of::<cera_hip_paged_evict>(), 48);
+        assert_eq!(size_of::<cera_hip_verify_draft>(), 80);
     }
 }

@@ -1,0 +1,252 @@
+"""Attention over a paged cache through the C ABI, against the definition in 64 bits (tolerances: paged_util.attn_ref)."""
+import numpy as np
+import pytest
+
+import paged_util as P
+from cera_amd import hip_api as A
+
+pytestmark = pytest.mark.gpu
+
+SCALE = {64: 0.125, 128: 128 ** -0.5}
+
+
+def _new_rows(pool, rows, lens, counts):
+    """The reference's cache with the call's own rows in it."""
+    at = 0
+    for s, (n, m) in enumerate(zip(lens, counts)):
+        if m and n:
+            pool.k[s][n - m:] = rows.k_new[at:at + m].astype(pool.dtype)
+            pool.v[s][n - m:] = rows.v_new[at:at + m].astype(pool.dtype)
+        at += m
+
+
+def _check(pool, rows, counts, window, sinks, got=None, skip=()):
+    got = rows.result() if got is None else got
+    at, masses = 0, []
+    for s, m in enumerate(counts):
+        if s not in skip:
+            out, bound, mass, mb = P.attn_ref(rows.q[at:at + m], pool.k[s], pool.v[s], m, 1 / np.sqrt(pool.hd), window, sinks)
+            bad = ~(np.abs(got[at:at + m] - out) <= bound)
+            assert not bad.any(), (s, np.argwhere(bad)[:4], np.abs(got[at:at + m] - out).max(), bound.max())
+            masses.append((mass, mb))
+        else:
+            masses.append(None)
+        at += m
+    return masses
+
+
+LENS = [0, 1, 2, 15, 16, 17, 31, 33, 64, 100, 255, 257, 700]
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("heads,n_kv,hd,page", [(32, 8, 128, 64), (28, 4, 128, 16), (12, 2, 64, 32), (4, 4, 64, 256), (8, 1, 128, 128), (18, 2, 64, 16), (20, 1, 128, 32)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4), (16, 0), (1, 33), (300, 70)])
+def test_one_token_of_every_sequence(hip, f16, heads, n_kv, hd, page, window, sinks):
+    print("decode", f16, heads, n_kv, hd, page, window, sinks, flush=True)
+    pool = P.Pool(hip, LENS, n_kv, hd, f16, page, seed=heads + page)
+    rows = P.Rows(pool, len(LENS), heads, seed=7, pad=8, new=True)
+    hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks))
+    _new_rows(pool, rows, LENS, [1] * len(LENS))
+    _check(pool, rows, [1] * len(LENS), window, sinks)
+    for s in (1, 5, len(LENS) - 1):    # what was written, bit for bit, and nothing else
+        k, v = pool.rows(s, LENS[s])
+        assert np.array_equal(k, pool.k[s]) and np.array_equal(v, pool.v[s])
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_a_long_sequence_beside_short_ones(hip, f16):
+    lens = [9001, 3, 5000, 1, 777]
+    pool = P.Pool(hip, lens, 2, 128, f16, 64, seed=3)
+    rows = P.Rows(pool, len(lens), 8, seed=4)
+    for window, sinks in ((0, 0), (2500, 5)):
+        hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks))
+        first = rows.result().copy()
+        _check(pool, rows, [1] * len(lens), window, sinks, first)
+        hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks, max_len=9001))
+        assert np.array_equal(first.view(np.uint32), rows.result().view(np.uint32))      # the same call again has the same bits
+    pool.close()
+
+
+@pytest.mark.parametrize("heads,n_kv,hd,f16", [(32, 8, 128, True), (14, 2, 64, True), (8, 2, 128, False), (20, 1, 64, True)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 6)])
+def test_weights_add_up_by_position(hip, heads, n_kv, hd, f16, window, sinks):
+    lens = [1, 0, 33, 700, 2600]
+    pool = P.Pool(hip, lens, n_kv, hd, f16, 32, seed=11)
+    cap = pool.cols * pool.page + 5
+    r = np.random.default_rng(5)
+    before = r.random((len(lens), n_kv, cap)).astype(np.float32)
+    d_mass = pool.dev(before)
+    rows = P.Rows(pool, len(lens), heads, seed=12, new=True)
+    _new_rows(pool, rows, lens, [1] * len(lens))
+    steps = 2
+    for _ in range(steps):
+        hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks, mass=d_mass, mass_stride=cap))
+    masses = _check(pool, rows, [1] * len(lens), window, sinks)
+    got = hip.download(d_mass, before.shape, np.float32)
+    for s, n in enumerate(lens):
+        mass, mb = masses[s]
+        want = before[s, :, :n] + steps * mass
+        if n:
+            want[:, n - 1] = mass[:, n - 1]        # the new position's weight starts at nothing, in each of the calls
+        bound = steps * mb + (steps + heads // n_kv) * 2.0 ** -24 * (want + 1)
+        assert (np.abs(got[s, :, :n] - want) <= bound).all()
+        assert np.array_equal(got[s, :, n:], before[s, :, n:])
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("heads,n_kv,hd,page", [(32, 8, 128, 64), (14, 2, 64, 16), (3, 1, 128, 32), (16, 16, 64, 128), (20, 2, 128, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (48, 4), (7, 0), (130, 40)])
+def test_chunks_of_new_tokens(hip, f16, heads, n_kv, hd, page, window, sinks):
+    print("chunk", f16, heads, n_kv, hd, page, window, sinks, flush=True)
+    lens, counts = [5, 64, 0, 333, 90, 17, 130], [5, 3, 0, 1, 77, 16, 65]
+    pool = P.Pool(hip, lens, n_kv, hd, f16, page, seed=heads, interleaved=True)
+    rows = P.Rows(pool, sum(counts), heads, seed=8, pad=4, new=True)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first), window=window, n_sink=sinks, max_queries=77))
+    _new_rows(pool, rows, lens, counts)
+    _check(pool, rows, counts, window, sinks)
+    for s, n in enumerate(lens):
+        k, v = pool.rows(s, n)
+        assert np.array_equal(k, pool.k[s]) and np.array_equal(v, pool.v[s])
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (200, 4)])
+def test_a_long_chunk(hip, f16, window, sinks):
+    lens, counts = [1500, 400], [300, 400]
+    pool = P.Pool(hip, lens, 2, 128, f16, 32, seed=2)
+    rows = P.Rows(pool, sum(counts), 8, seed=9)
+    first = np.array([0, 300, 700], np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first), window=window, n_sink=sinks))
+    _check(pool, rows, counts, window, sinks)
+    pool.close()
+
+
+def test_rows_of_no_sequence_stay(hip):
+    pool = P.Pool(hip, [40, 20], 2, 64, True, 16, seed=2)
+    rows = P.Rows(pool, 12, 4, seed=9)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(np.array([2, 5, 9], np.uint32))))
+    got = rows.result()
+    assert (got[:2] == P.SENTINEL).all() and (got[9:] == P.SENTINEL).all()
+    for s, (a, b) in enumerate(((2, 5), (5, 9))):
+        out, bound, _, _ = P.attn_ref(rows.q[a:b], pool.k[s], pool.v[s], b - a, 0.125, 0, 0)
+        assert (np.abs(got[a:b] - out) <= bound).all()
+    pool.close()
+
+
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("f16", [True, False])
+def test_bad_pages_and_lengths_give_nan_to_their_own_sequence(hip, chunk, f16):
+    lens = [40, 70, 300, 33, 20]
+    pool = P.Pool(hip, lens, 2, 64, f16, 16, seed=6)
+    rows = P.Rows(pool, len(lens), 4, seed=3, new=True)
+    table = pool.table.copy()
+    table[0, 1], table[2, 0], table[4, 0] = -1, pool.n_pages, 0x7FFFFFFF
+    bad_lens = np.array(lens, np.uint32)
+    bad_lens[3] = pool.cols * pool.page + 1
+    kv = pool.kv(table=pool.dev(table), lens=pool.dev(bad_lens))
+    more = dict(q_first=pool.dev(np.arange(len(lens) + 1, dtype=np.uint32))) if chunk else {}
+    hip.paged_attn(kv, rows.op(**more))
+    _new_rows(pool, rows, lens, [1] * len(lens))
+    got = rows.result()
+    for s in (0, 2, 3, 4):
+        assert np.isnan(got[s]).all(), s
+    _check(pool, rows, [1] * len(lens), 0, 0, got, skip=(0, 2, 3, 4))
+    # behind a window the bad first page is out of sight
+    hip.paged_attn(kv, rows.op(window=16, **more))
+    got = rows.result()
+    out, bound, _, _ = P.attn_ref(rows.q[2:3], pool.k[2], pool.v[2], 1, 0.125, 16, 0)
+    assert (np.abs(got[2:3] - out) <= bound).all() and np.isnan(got[3]).all()
+    pool.close()
+
+
+def test_rows_out_of_order_give_nan(hip):
+    pool = P.Pool(hip, [40, 20, 30, 8], 2, 64, True, 16, seed=2)
+    rows = P.Rows(pool, 20, 4, seed=9, new=True)
+    before = pool.pages()
+    # rows that decrease, more rows than positions, more than max_queries, an end behind n_rows
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(np.array([3, 1, 8, 11, 21], np.uint32)), max_queries=6))
+    got = rows.result()
+    assert np.isnan(got[1:8]).all() and np.isnan(got[11:]).all() and (got[0] == P.SENTINEL).all()
+    out, bound, _, _ = P.attn_ref(rows.q[8:11], np.concatenate([pool.k[2][:27], rows.k_new[8:11].astype(np.float16)]),
+                                  np.concatenate([pool.v[2][:27], rows.v_new[8:11].astype(np.float16)]), 3, 0.125, 0, 0)
+    assert (np.abs(got[8:11] - out) <= bound).all()
+    after = pool.pages()
+    for s in (0, 1, 3):
+        for t in range(pool.lens[s]):
+            p = pool.table[s, t // 16]
+            for x, y in zip(before, after):
+                assert np.array_equal(x[p, :, t % 16], y[p, :, t % 16])
+    pool.close()
+
+
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("f16", [True, False])
+def test_large_and_small_queries(hip, f16, chunk):
+    """Queries far from 1 lose nothing to their halves, and none are zeros."""
+    lens = [70] * 5
+    pool = P.Pool(hip, lens, 1, 64, f16, 16, seed=6)
+    rows = P.Rows(pool, 5, 2, seed=3)
+    for s, f in enumerate((1e-20, 300, 1e4, 0, 1e-3)):
+        rows.q[s] *= np.float32(f)
+    hip.upload(rows.d_q, rows.q)
+    hip.paged_attn(pool.kv(), rows.op(**(dict(q_first=pool.dev(np.arange(6, dtype=np.uint32))) if chunk else {})))
+    _check(pool, rows, [1] * 5, 0, 0)
+    pool.close()
+
+
+def test_offsets_beyond_32_bits(hip):
+    """Pages 2^31 elements apart: byte and element offsets past 32 bits."""
+    stride, n_kv, hd, page = (1 << 31) + 8, 2, 128, 16
+    base = hip.malloc(3 * stride * 2)
+    r = np.random.default_rng(0)
+    n = 40
+    k, v = (r.standard_normal((n, n_kv, hd)).astype(np.float16) for _ in range(2))
+    table = np.array([[2, 0, 1]], np.int32)
+    per = n_kv * page * hd
+    for i, p in enumerate(table[0]):
+        for x, off in ((k, 0), (v, per)):
+            block = np.zeros((n_kv, page, hd), np.float16)
+            part = x[i * page:(i + 1) * page]
+            block[:, :len(part)] = part.transpose(1, 0, 2)
+            hip.upload(base + (int(p) * stride + off) * 2, block)
+    q = r.standard_normal((1, 8, hd)).astype(np.float32)
+    bufs = [hip.to_device(x) for x in (table, np.array([n], np.uint32), q)]
+    d_out = hip.malloc(q.nbytes)
+    hip.paged_attn(A.PagedKV(kv_type=1, n_kv_heads=n_kv, head_dim=hd, page_size=page, n_pages=3, n_seqs=1, max_pages=3, page_stride=stride, k=base, v=base + per * 2,
+                             table=bufs[0], lens=bufs[1]), A.PagedAttn(q=bufs[2], out=d_out, n_rows=1, n_heads=8, scale=SCALE[hd]))
+    got = hip.download(d_out, q.shape, np.float32)
+    out, bound, _, _ = P.attn_ref(q, k, v, 1, SCALE[hd], 0, 0)
+    assert (np.abs(got - out) <= bound).all()
+    for b in bufs + [d_out, base]:
+        hip.free(b)
+
+
+def test_sequences_that_share_pages(hip):
+    """Two sequences with the same first pages: reading them needs no copies."""
+    pool = P.Pool(hip, [96, 96], 2, 64, True, 32, seed=1)
+    table = pool.table.copy()
+    table[1, :2] = table[0, :2]
+    rows = P.Rows(pool, 2, 4, seed=3)
+    hip.paged_attn(pool.kv(table=pool.dev(table)), rows.op())
+    for x in (pool.k, pool.v):
+        x[1][:64] = x[0][:64]
+    _check(pool, rows, [1, 1], 0, 0)
+    pool.close()
+
+
+def test_refusals(hip):
+    pool = P.Pool(hip, [40, 20], 2, 64, True, 16, seed=2)
+    rows = P.Rows(pool, 2, 4, seed=9)
+    for kv, op, status in ((pool.kv(head_dim=96), rows.op(), 4), (pool.kv(page_size=24), rows.op(), 4), (pool.kv(kv_type=2), rows.op(), 3), (pool.kv(), rows.op(n_heads=3), 4),
+                           (pool.kv(), rows.op(out=None), 6), (pool.kv(), rows.op(scale=float("nan")), 6), (pool.kv(), rows.op(q=rows.d_q + 4), 6), (pool.kv(), rows.op(n_rows=1), 4),
+                           (pool.kv(), rows.op(k_new=rows.d_q), 6), (pool.kv(k=None), rows.op(), 6)):
+        with pytest.raises(A.HipError) as e:
+            hip.paged_attn(kv, op)
+        assert e.value.status == status and e.value.message
+    assert (rows.result() == P.SENTINEL).all()
+    hip.paged_attn(pool.kv(n_seqs=0), rows.op(n_rows=0))
+    pool.close()
