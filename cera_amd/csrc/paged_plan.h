@@ -122,3 +122,23 @@ PAGED_HD PagedSeen paged_seen(uint32_t P, uint32_t window, uint32_t n_sink) {
     v.sink_end = n_sink < v.start ? n_sink : v.start;
     return v;
 }
+
+// How a sequence's tiles are cut into parts, a workgroup each.  groups: workgroups of a part over all sequences.
+struct PagedCut {
+    uint32_t part_tiles, max_parts;
+};
+inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint64_t groups, uint32_t n_cu) {
+    // tiles that a sequence of max_len may have: those of the window and of the first positions each touch one more at their ends
+    uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
+    if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
+    most = std::max<uint64_t>(most, 1);
+    // enough workgroups for four a CU, of at least two tiles a wavefront and at most 1024 positions
+    const uint64_t want = std::max<uint64_t>(1, 4ull * n_cu / std::max<uint64_t>(groups, 1));
+    uint64_t tiles = std::max<uint64_t>(8, (most + want - 1) / want);
+    tiles = std::min<uint64_t>((tiles + 3) / 4 * 4, std::max<uint64_t>(1024 / tile, 8));
+    tiles = std::max<uint64_t>(tiles, ((most + 1023) / 1024 + 3) / 4 * 4);   // and at most 1024 of them
+    PagedCut c;
+    c.part_tiles = static_cast<uint32_t>(tiles);
+    c.max_parts = static_cast<uint32_t>((most + tiles - 1) / tiles);
+    return c;
+}

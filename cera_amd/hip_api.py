@@ -118,7 +118,7 @@ class PagedAttn(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("q", "k_new", "v_new", "out", "mass", "q_first")] + \
                [(n, C.c_uint64) for n in ("q_stride", "kv_stride", "out_stride", "mass_stride")] + \
                [(n, C.c_uint32) for n in ("n_rows", "max_queries", "n_heads")] + [("scale", C.c_float)] + \
-               [(n, C.c_uint32) for n in ("window", "n_sink", "max_len", "_reserved")]
+               [(n, C.c_uint32) for n in ("window", "n_sink", "max_len", "mass_fresh")]
 
 
 class PagedEvict(C.Structure):

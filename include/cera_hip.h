@@ -504,7 +504,8 @@ typedef struct {
  * f32, which are written into the pages first (narrowed to half to the nearest even) and so have to
  * be in pages of their own sequence only.
  * mass (nullable, decode form): mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
- * g's query heads of the softmax weight of position t; with k_new, the new position's starts at 0.
+ * g's query heads of the softmax weight of position t.  With k_new and mass_fresh the new position's
+ * starts at 0, whatever an eviction or a shortened sequence has left there.
  * Memory: mass and many parts take a workspace of the context (about 4 bytes * n_heads * max_len per
  * sequence for mass).  Results do not depend on other sequences of the call or on earlier calls.
  * Host refusals: n_heads not a multiple of n_kv_heads, scale not finite, pointers not 16-byte (lens,
@@ -524,7 +525,7 @@ typedef struct {
     uint32_t n_rows, max_queries, n_heads;
     float scale;
     uint32_t window, n_sink;
-    uint32_t max_len, _reserved;
+    uint32_t max_len, mass_fresh;
 } cera_hip_paged_attn;
 CERA_HIP_API cera_hip_status cera_hip_paged_attn_dev(cera_hip_ctx*, const cera_hip_paged_kv*, const cera_hip_paged_attn*);
 

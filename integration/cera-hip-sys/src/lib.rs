@@ -290,7 +290,7 @@ pub struct cera_hip_paged_attn {
     pub window: u32,
     pub n_sink: u32,
     pub max_len: u32,
-    pub _reserved: u32,
+    pub mass_fresh: u32,
 }
 
 /// Eviction from a paged cache by accumulated attention weight.

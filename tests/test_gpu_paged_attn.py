@@ -69,8 +69,8 @@ def test_a_long_sequence_beside_short_ones(hip, f16):
 
 
 @pytest.mark.parametrize("heads,n_kv,hd,f16", [(32, 8, 128, True), (14, 2, 64, True), (8, 2, 128, False), (20, 1, 64, True)])
-@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 6)])
-def test_weights_add_up_by_position(hip, heads, n_kv, hd, f16, window, sinks):
+@pytest.mark.parametrize("window,sinks,fresh", [(0, 0, 0), (0, 0, 1), (100, 6, 1)])
+def test_weights_add_up_by_position(hip, heads, n_kv, hd, f16, window, sinks, fresh):
     lens = [1, 0, 33, 700, 2600]
     pool = P.Pool(hip, lens, n_kv, hd, f16, 32, seed=11)
     cap = pool.cols * pool.page + 5
@@ -81,13 +81,13 @@ def test_weights_add_up_by_position(hip, heads, n_kv, hd, f16, window, sinks):
     _new_rows(pool, rows, lens, [1] * len(lens))
     steps = 2
     for _ in range(steps):
-        hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks, mass=d_mass, mass_stride=cap))
+        hip.paged_attn(pool.kv(), rows.op(window=window, n_sink=sinks, mass=d_mass, mass_stride=cap, mass_fresh=fresh))
     masses = _check(pool, rows, [1] * len(lens), window, sinks)
     got = hip.download(d_mass, before.shape, np.float32)
     for s, n in enumerate(lens):
         mass, mb = masses[s]
         want = before[s, :, :n] + steps * mass
-        if n:
+        if n and fresh:
             want[:, n - 1] = mass[:, n - 1]        # the new position's weight starts at nothing, in each of the calls
         bound = steps * mb + (steps + heads // n_kv) * 2.0 ** -24 * (want + 1)
         assert (np.abs(got[s, :, :n] - want) <= bound).all()
