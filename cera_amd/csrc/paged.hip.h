@@ -24,6 +24,16 @@ static inline PagedView paged_view(const cera_hip_paged_kv& c, uint32_t max_len)
     return v;
 }
 
+// What no kernel of the call writes, by scalar loads where the index is the same in all lanes: a vector load's wait is one for all
+// loads in flight before it.
+template <typename T> using PagedConst = const __attribute__((address_space(4))) T*;
+template <typename T> __device__ __forceinline__ PagedConst<T> paged_const(const T* p) { return (PagedConst<T>)p; }
+
+__device__ __forceinline__ PagedRows paged_rows(const uint32_t* q_first, const uint32_t* lens, uint32_t s, uint32_t n_rows, uint32_t max_queries, uint32_t max_len) {
+    const uint32_t len = paged_const(lens)[s];
+    return q_first ? paged_chunk_rows(paged_const(q_first)[s], paged_const(q_first)[s + 1], len, n_rows, max_queries, max_len) : paged_one_row(s, len, max_len);
+}
+
 // The page of position t (t < max_len, so the table has its column); *ok turns false where the table names none of the pool's, and the
 // page is then 0, whose memory is there.
 __device__ __forceinline__ uint32_t paged_page(const PagedView& v, uint32_t seq, uint32_t t, bool& ok) {

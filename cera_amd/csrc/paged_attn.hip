@@ -4,12 +4,12 @@
 #include "paged.hip.h"
 #include "paged_attn.hip.h"
 
-// ---- the new rows into their pages ---------------------------------------------------------------------------------
+// ---- chunks: the new rows into their pages -----------------------------------------------------------------------------
 // grid = (blocks, sequences); a thread moves four floats of a row's keys and values
 template <typename KV, int HD>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, const float* __restrict__ k_new,
                                                            const float* __restrict__ v_new, uint64_t kv_stride, const uint32_t* __restrict__ q_first,
-                                                           uint32_t n_rows, uint32_t max_queries, float* __restrict__ mass, uint64_t mass_stride) {
+                                                           uint32_t n_rows, uint32_t max_queries) {
     const uint32_t s = blockIdx.y;
     const PagedRows r = paged_rows(q_first, c.lens, s, n_rows, max_queries, c.max_len);
     if (r.bad || r.len == 0) return;
@@ -24,72 +24,108 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __re
         const uint64_t dst = paged_row<HD>(c, page, g, t), src = (r.first + static_cast<uint64_t>(row)) * kv_stride + g * HD;
         KvOps<KV>::st4(kp + dst, c4, *reinterpret_cast<const float4*>(k_new + src + 4 * c4));
         KvOps<KV>::st4(vp + dst, c4, *reinterpret_cast<const float4*>(v_new + src + 4 * c4));
-        if (mass && c4 == 0) mass[(static_cast<uint64_t>(s) * c.n_kv + g) * mass_stride + t] = 0.0f;
     }
 }
 
-// ---- the parts of a sequence joined --------------------------------------------------------------------------------
-// grid = (kv heads * column groups, columns of a group, sequences), HD / 4 threads: four values each
-template <int HD>
-__global__ __launch_bounds__(64) void paged_merge_kernel(PagedView c, PagedOp a) {
-    const uint32_t g = blockIdx.x / a.n_cg, cg = blockIdx.x % a.n_cg, s = blockIdx.z, d = threadIdx.x * 4;
+// ---- the parts of a sequence joined, and weights added up by position ------------------------------------------------
+// grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 2048 positions of a kv head each.
+// Columns: HD / 4 threads of four values for each of SPLIT shares of a column's parts.  Positions: the scores lie as the attention
+// left them, in the base-2 domain.
+static constexpr uint32_t PAGED_MASS_POS = 2048;
+// part p of a sequence lies this many slots behind slot 2 (its first workgroup)
+__device__ __forceinline__ uint64_t paged_slot(uint32_t p) { return p == 0 ? 1 : 2 * static_cast<uint64_t>(p); }
+template <int HD, int SPLIT>
+__global__ __launch_bounds__(256) void paged_finish_kernel(PagedView c, PagedOp a, uint32_t merge_blocks, uint32_t mass_blocks) {
+    constexpr uint32_t COLS = 256 / (HD / 4 * SPLIT);
+    __shared__ __attribute__((aligned(16))) float4 s_o[SPLIT > 1 ? 256 : 1];
+    __shared__ float s_m[SPLIT > 1 ? 256 : 1], s_l[SPLIT > 1 ? 256 : 1];
+    extern __shared__ float s_h[];   // [G] maximum, [G] 1 / sum
+    const uint32_t s = blockIdx.y, tid = threadIdx.x;
     const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
     if (r.bad || r.len == 0) return;   // written by the attention's launch
-    const uint32_t n_cols = r.n * a.G, col = cg * a.n_cols + blockIdx.y;
-    if (col >= n_cols) return;
-    const PagedTiles t = paged_tiles(r, cg * a.n_cols, min(cg * a.n_cols + a.n_cols, n_cols) - 1, a);
-    const uint32_t parts = (t.n + a.part_tiles - 1) / a.part_tiles;
-    if (parts <= 1 || threadIdx.x >= HD / 4) return;
-    const uint64_t first = ((static_cast<uint64_t>(s) * gridDim.x + blockIdx.x) * a.max_parts) * a.n_cols + blockIdx.y;
-    float M = PAGED_LOWEST;
-    for (uint32_t p = 0; p < parts; ++p) M = fmaxf(M, a.ml[(first + static_cast<uint64_t>(p) * a.n_cols) * 2]);
-    float L = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (uint32_t p = 0; p < parts; ++p) {
-        const uint64_t at = first + static_cast<uint64_t>(p) * a.n_cols;
-        const float f = __builtin_amdgcn_exp2f(a.ml[at * 2] - M);
-        const float4 x = *reinterpret_cast<const float4*>(a.acc + at * HD + d);
-        L = fmaf(f, a.ml[at * 2 + 1], L);
-        o.x = fmaf(f, x.x, o.x); o.y = fmaf(f, x.y, o.y); o.z = fmaf(f, x.z, o.z); o.w = fmaf(f, x.w, o.w);
+    const uint32_t n_cols = r.n * a.G;
+    if (blockIdx.x < merge_blocks) {
+        const uint32_t blocks = (a.n_cols + COLS - 1) / COLS, gx = blockIdx.x / blocks, g = gx / a.n_cg, cg = gx % a.n_cg;
+        const uint32_t x = tid % (HD / 4), share = tid / (HD / 4) % SPLIT, lcol = blockIdx.x % blocks * COLS + tid / (HD / 4 * SPLIT), col = cg * a.n_cols + lcol;
+        if (cg * a.n_cols >= n_cols) return;
+        const uint2 cut = a.cut[static_cast<uint64_t>(gx) * gridDim.y + s];
+        const uint32_t parts = cut.y - cut.x + 1;
+        if (parts == 1) return;
+        const bool mine = lcol < a.n_cols && col < n_cols;
+        const uint64_t first = (static_cast<uint64_t>(gx) * 2 * a.spans + 2 * cut.x) * a.n_cols + (mine ? lcol : 0);
+        float M = PAGED_LOWEST;
+        for (uint32_t p = share; p < parts; p += SPLIT) M = fmaxf(M, a.ml[(first + paged_slot(p) * a.n_cols) * 2]);
+        float L = 0.0f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (uint32_t p = share; p < parts; p += SPLIT) {
+            const uint64_t at = first + paged_slot(p) * a.n_cols;
+            const float f = __builtin_amdgcn_exp2f(a.ml[at * 2] - M);
+            const float4 y = *reinterpret_cast<const float4*>(a.acc + at * HD + 4 * x);
+            L = fmaf(f, a.ml[at * 2 + 1], L);
+            o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
+        }
+        if constexpr (SPLIT > 1) {
+            s_o[tid] = o;
+            s_m[tid] = M;
+            s_l[tid] = L;
+            __syncthreads();
+            if (share) return;
+            for (uint32_t i = 1; i < SPLIT; ++i) M = fmaxf(M, s_m[tid + i * (HD / 4)]);
+            L = 0.0f;
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (uint32_t i = 0; i < SPLIT; ++i) {
+                const uint32_t u = tid + i * (HD / 4);
+                const float f = __builtin_amdgcn_exp2f(s_m[u] - M);
+                const float4 y = s_o[u];
+                L = fmaf(f, s_l[u], L);
+                o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
+            }
+        }
+        if (!mine) return;
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
+        *reinterpret_cast<float4*>(a.out + (r.first + static_cast<uint64_t>(col / a.G)) * a.out_stride + (g * a.G + col % a.G) * HD + 4 * x) = o;
+        return;
     }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
-    *reinterpret_cast<float4*>(a.out + (r.first + static_cast<uint64_t>(col / a.G)) * a.out_stride + (g * a.G + col % a.G) * HD + d) = o;
-}
-
-// ---- weights added up by position ----------------------------------------------------------------------------------
-// grid = (blocks of positions, kv heads, sequences).  The scores lie as the attention left them, in the base-2 domain.
-__global__ __launch_bounds__(256) void paged_mass_kernel(PagedView c, PagedOp a) {
-    extern __shared__ float sh[];   // [G] maximum, [G] 1 / sum
-    const uint32_t g = blockIdx.y, s = blockIdx.z;
-    const PagedRows r = paged_rows(nullptr, c.lens, s, a.n_rows, 1, c.max_len);
-    if (r.bad || r.len == 0) return;
-    const uint32_t P = r.len - 1;
+    const uint32_t g = (blockIdx.x - merge_blocks) / mass_blocks, i0 = (blockIdx.x - merge_blocks) % mass_blocks * PAGED_MASS_POS, P = r.len - 1;
     const PagedSeen v = paged_seen(P, a.window, a.n_sink);
     const uint32_t n_seen = v.sink_end + (P + 1 - v.start);
-    if (blockIdx.x * 1024u >= n_seen) return;
-    for (uint32_t h = threadIdx.x; h < a.G; h += 256) {
-        const uint32_t cg = h / a.n_cols, last = min(cg * a.n_cols + a.n_cols, a.G) - 1;
-        const PagedTiles t = paged_tiles(r, cg * a.n_cols, last, a);
-        const uint32_t parts = (t.n + a.part_tiles - 1) / a.part_tiles;
-        const uint64_t first = ((static_cast<uint64_t>(s) * c.n_kv * a.n_cg + g * a.n_cg + cg) * a.max_parts) * a.n_cols + h % a.n_cols;
+    if (i0 >= n_seen) return;
+    for (uint32_t h = tid >> 6; h < a.G; h += 4) {   // a wavefront per head, its lanes over the parts
+        const uint32_t cg = h / a.n_cols;
+        const uint64_t gx = g * a.n_cg + cg;
+        const uint2 cut = a.spans ? a.cut[gx * gridDim.y + s] : make_uint2(0, 0);
         float M = PAGED_LOWEST, L = 0.0f;
-        for (uint32_t p = 0; p < parts; ++p) M = fmaxf(M, a.ml[(first + static_cast<uint64_t>(p) * a.n_cols) * 2]);
-        for (uint32_t p = 0; p < parts; ++p) {
-            const uint64_t at = first + static_cast<uint64_t>(p) * a.n_cols;
-            L = fmaf(__builtin_amdgcn_exp2f(a.ml[at * 2] - M), a.ml[at * 2 + 1], L);
+        if (cut.x == cut.y) {
+            const float* const ml = a.ml_seq + ((gx * gridDim.y + s) * a.n_cols + h % a.n_cols) * 2;
+            M = ml[0];
+            L = ml[1];
+        } else {
+            const uint64_t first = (gx * 2 * a.spans + 2 * cut.x) * a.n_cols + h % a.n_cols;
+            for (uint32_t p = tid & 63; p <= cut.y - cut.x; p += 64) M = fmaxf(M, a.ml[(first + paged_slot(p) * a.n_cols) * 2]);
+            M = wave_max(M);
+            for (uint32_t p = tid & 63; p <= cut.y - cut.x; p += 64) {
+                const uint64_t at = first + paged_slot(p) * a.n_cols;
+                L = fmaf(__builtin_amdgcn_exp2f(a.ml[at * 2] - M), a.ml[at * 2 + 1], L);
+            }
+            L = wave_sum(L);
         }
-        sh[h] = M - PAGED_P_LOG2;
-        sh[a.G + h] = L == 0.0f ? 0.0f : 1.0f / L;   // NaN where a page was bad
+        if ((tid & 63) == 0) {
+            s_h[h] = M - PAGED_P_LOG2;
+            s_h[a.G + h] = L == 0.0f ? 0.0f : 1.0f / L;   // NaN where a page was bad
+        }
     }
     __syncthreads();
     float* const m = a.mass + (static_cast<uint64_t>(s) * c.n_kv + g) * a.mass_stride;
-    for (uint32_t i = blockIdx.x * 1024u + threadIdx.x; i < min(n_seen, blockIdx.x * 1024u + 1024u); i += 256) {
+    const float* const sc = a.scores + (static_cast<uint64_t>(s) * c.n_kv + g) * a.G * a.score_stride;
+    for (uint32_t i = i0 + tid; i < min(n_seen, i0 + PAGED_MASS_POS); i += 256) {
         const uint32_t t = i < v.sink_end ? i : v.start + (i - v.sink_end);
+        const float before = a.mass_fresh && t == P ? 0.0f : m[t];
         float sum = 0.0f;
-        for (uint32_t h = 0; h < a.G; ++h)
-            sum = fmaf(__builtin_amdgcn_exp2f(a.scores[(static_cast<uint64_t>(s) * c.n_kv * a.G + g * a.G + h) * a.score_stride + t] - sh[h]), sh[a.G + h], sum);
-        if (sum == sum) m[t] += sum;
+        for (uint32_t h = 0; h < a.G; ++h) sum = fmaf(__builtin_amdgcn_exp2f(sc[h * a.score_stride + t] - s_h[h]), s_h[a.G + h], sum);
+        if (sum == sum) m[t] = before + sum;
     }
 }
 
@@ -101,7 +137,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.q = in.q; a.out = in.out; a.mass = in.mass; a.q_first = in.q_first;
     a.q_stride = in.q_stride ? in.q_stride : static_cast<uint64_t>(in.n_heads) * HD;
     a.out_stride = in.out_stride ? in.out_stride : static_cast<uint64_t>(in.n_heads) * HD;
+    a.kv_stride = in.kv_stride ? in.kv_stride : static_cast<uint64_t>(c.n_kv_heads) * HD;
     a.mass_stride = in.mass_stride;
+    a.mass_fresh = in.k_new && in.mass_fresh;
     a.n_rows = in.n_rows;
     a.max_queries = in.q_first ? (in.max_queries ? std::min(in.max_queries, in.n_rows) : in.n_rows) : 1;
     a.G = in.n_heads / c.n_kv_heads;
@@ -113,47 +151,53 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
     if (static_cast<uint64_t>(c.n_kv_heads) * a.n_cg > (1u << 23)) return cera_fail(ctx, CERA_HIP_ERR_SHAPE, "paged attention: too many rows of a sequence for one call");
     a.tile = HALF ? 32 : 16;
-    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, static_cast<uint64_t>(c.n_seqs) * c.n_kv_heads * a.n_cg, ctx->n_cu);
-    a.part_tiles = cut.part_tiles;
-    a.max_parts = cut.max_parts;
+    const uint32_t wide = c.n_kv_heads * a.n_cg;
+    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, ctx->n_cu);
+    a.spans = cut.spans;
+    a.least = cut.least;
     a.score_stride = a.mass ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;
-    auto bytes = [&](uint64_t parts) {
-        const uint64_t n = parts > 1 || a.mass ? static_cast<uint64_t>(c.n_seqs) * c.n_kv_heads * a.n_cg * parts * a.n_cols : 0;
-        return n * (parts > 1 ? HD + 2 : 2) * 4 + a.score_stride * c.n_seqs * in.n_heads * 4;
-    };
+    // scores | results of parts | maxima and sums of parts | of whole sequences | who has a sequence's parts
+    const uint64_t scores = a.score_stride * c.n_seqs * in.n_heads, seqs = static_cast<uint64_t>(wide) * c.n_seqs, ml_seq = a.mass ? seqs * a.n_cols * 2 : 0;
+    auto parts = [&] { return static_cast<uint64_t>(wide) * 2 * a.spans * a.n_cols; };
+    auto bytes = [&] { return 4 * (scores + parts() * (HD + 2) + ml_seq + (a.spans ? 2 * seqs : 0)); };
     void* ws = nullptr;
-    if (a.max_parts > 1) {
-        CERA_TRY(cera_scratch_if_room(ctx, 15, bytes(a.max_parts), &ws));
-        if (!ws) {   // one workgroup walks all of a sequence
-            a.max_parts = 1;
-            a.part_tiles = 0x7FFFFFFFu;
-        }
+    if (a.spans) {
+        CERA_TRY(cera_scratch_if_room(ctx, 15, bytes(), &ws));
+        if (!ws) a.spans = 0;
     }
-    if (!ws && bytes(a.max_parts)) CERA_TRY(cera_scratch(ctx, 15, bytes(a.max_parts), &ws));
+    if (!ws && bytes()) CERA_TRY(cera_scratch(ctx, 15, bytes(), &ws));
     a.scores = static_cast<float*>(ws);
-    a.ml = a.scores + a.score_stride * c.n_seqs * in.n_heads;
-    a.acc = a.ml + static_cast<uint64_t>(c.n_seqs) * c.n_kv_heads * a.n_cg * a.max_parts * a.n_cols * 2;
-    if (in.k_new) {
+    a.acc = a.scores + scores;
+    a.ml = a.acc + parts() * HD;
+    a.ml_seq = a.ml + parts() * 2;
+    a.cut = reinterpret_cast<uint2*>(a.ml_seq + ml_seq);
+    if (in.k_new && in.q_first) {
         const uint64_t items = static_cast<uint64_t>(a.max_queries) * c.n_kv_heads * (HD / 4);
         hipLaunchKernelGGL((paged_append_kernel<KV, HD>), dim3(static_cast<uint32_t>(std::min<uint64_t>((items + 255) / 256, 1024)), c.n_seqs), dim3(256), 0, ctx->stream, v,
-                           static_cast<KV*>(c.k), static_cast<KV*>(c.v), in.k_new, in.v_new, in.kv_stride ? in.kv_stride : static_cast<uint64_t>(c.n_kv_heads) * HD, a.q_first, a.n_rows,
-                           a.max_queries, in.mass_fresh ? a.mass : nullptr, a.mass_stride);
+                           static_cast<KV*>(c.k), static_cast<KV*>(c.v), in.k_new, in.v_new, a.kv_stride, a.q_first, a.n_rows, a.max_queries);
+    } else {
+        a.k_new = in.k_new;
+        a.v_new = in.v_new;
     }
-    const dim3 grid(c.n_kv_heads * a.n_cg, a.max_parts, c.n_seqs);
+    const dim3 grid(wide, a.spans ? a.spans : c.n_seqs);
     auto launch = [&](auto tag) {
         constexpr int CB = decltype(tag)::value;
-        if (a.mass) hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, true>), grid, dim3(256), 0, ctx->stream, v, static_cast<const KV*>(c.k), static_cast<const KV*>(c.v), a);
-        else hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, false>), grid, dim3(256), 0, ctx->stream, v, static_cast<const KV*>(c.k), static_cast<const KV*>(c.v), a);
+        if (a.mass) hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, true>), grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
+        else hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, false>), grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
     };
     if (cb == 2) {
         if constexpr (HALF) launch(std::integral_constant<int, 2>{});
     } else {
         launch(std::integral_constant<int, 1>{});
     }
-    if (a.max_parts > 1) hipLaunchKernelGGL((paged_merge_kernel<HD>), dim3(c.n_kv_heads * a.n_cg, a.n_cols, c.n_seqs), dim3(64), 0, ctx->stream, v, a);
-    if (a.mass) {
+    if (a.spans || a.mass) {
+        const bool many = a.spans > 8;   // parts of a column shared out
+        const uint32_t cols_wg = 256 / (HD / 4 * (many ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
-        hipLaunchKernelGGL(paged_mass_kernel, dim3(static_cast<uint32_t>((most + 1023) / 1024), c.n_kv_heads, c.n_seqs), dim3(256), a.G * 8, ctx->stream, v, a);
+        const uint32_t mass = a.mass ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;
+        const dim3 blocks(merge + mass * c.n_kv_heads, c.n_seqs);
+        if (many) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
+        else hipLaunchKernelGGL((paged_finish_kernel<HD, 1>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
     }
     HIP_TRY(ctx, hipGetLastError());
     return CERA_HIP_OK;

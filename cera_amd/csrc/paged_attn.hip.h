@@ -26,10 +26,16 @@ struct PagedOp {
     uint32_t n_rows, max_queries, G;
     float scale2;   // times log2 e
     uint32_t window, n_sink;
+    const float *k_new, *v_new;              // decode form: the rows' own keys and values, or null
+    uint64_t kv_stride;
+    uint32_t mass_fresh;
     uint32_t n_cols, n_cg;                   // columns of a workgroup, groups of them a kv head
-    uint32_t tile, part_tiles, max_parts;    // positions of a tile, tiles of a part
-    float *acc, *ml;                         // [seq][kv head][group][part][column] x [HD], x (maximum, sum)
-    float* scores;                           // [seq][head][score_stride]
+    uint32_t tile;                           // positions of a tile
+    uint32_t spans, least;                   // workgroups of a kv head and group, and their least number of tiles; spans 0: one for each sequence
+    float *acc, *ml;                         // [kv head, group][2 spans][column] x [HD], x (maximum, sum)
+    uint2* cut;                              // [kv head, group][seq]: first and last workgroup of a sequence that is cut
+    float* ml_seq;                           // with mass: [kv head, group][seq][column] x (maximum, sum) of a sequence that is not
+    float* scores;                           // with mass: [seq][head][score_stride]
     uint64_t score_stride;
 };
 
@@ -49,6 +55,15 @@ __device__ __forceinline__ PagedTiles paged_tiles(const PagedRows& r, uint32_t c
     t.sinks = min((hi.sink_end + a.tile - 1) / a.tile, t.main);
     t.n = t.sinks + t.P_hi / a.tile - t.main + 1;
     return t;
+}
+
+// Tiles of sequence s for the columns from c0 on: none where it has no such columns; where nothing can be read, one for the first
+// columns' workgroup, which writes the rows.
+__device__ __forceinline__ uint32_t paged_count(const PagedView& c, const PagedOp& a, uint32_t s, uint32_t c0) {
+    const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
+    if (r.bad || r.len == 0) return c0 == 0;
+    const uint32_t n_cols = r.n * a.G;
+    return c0 < n_cols ? paged_tiles(r, c0, min(c0 + a.n_cols, n_cols) - 1, a).n : 0;
 }
 
 __device__ __forceinline__ float paged_xor_max(float v) {   // over the four lanes of a column
@@ -73,39 +88,128 @@ template <int HD> struct PagedTile<float, HD> {
     float4 v[4][VW];
 };
 
+template <int NC, int HD> struct PagedShared {
+    __attribute__((aligned(16))) float o[4][NC][HD + 4];
+    float m[4][NC], l[4][NC];
+};
+
+// Tiles [j_begin, j_end) of sequence s for one group of columns, by a workgroup of four wavefronts; slot: of a part's results.
 template <typename KV, int HD, int CB, bool MASS>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const KV* __restrict__ kp, const KV* __restrict__ vp, PagedOp a) {
+__device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8 : 16) * CB, HD>& sh, const PagedView& c, KV* __restrict__ kp, KV* __restrict__ vp, const PagedOp& a, uint32_t g,
+                                                uint32_t cg, uint32_t s, const PagedRows& r, const PagedTiles& tiles, uint32_t c0, uint32_t c_last, uint32_t j_begin, uint32_t j_end, uint32_t slot) {
     constexpr bool HALF = sizeof(KV) == 2;
     using Tile = PagedTile<KV, HD>;
     constexpr int POS = Tile::POS, SUB = Tile::SUB, KS = Tile::KS, NS = 4 * SUB;   // NS: scores of a lane and column block
     constexpr int CW = HALF ? 8 : 16, NC = CW * CB;
     constexpr int NO = HD / 16;                                                    // 16-row tiles of O^T
-    constexpr int OLD = HD + 4;
-    __shared__ __attribute__((aligned(16))) float s_o[4][NC][OLD];
-    __shared__ float s_m[4][NC], s_l[4][NC];
-
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid >> 6)));
-    const uint32_t g = blockIdx.x / a.n_cg, cg = blockIdx.x % a.n_cg, part = blockIdx.y, s = blockIdx.z;
-    const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
-    const uint32_t c0 = cg * NC;
-    if (r.bad || r.len == 0) {
-        // nothing is known of these rows but where they are
-        if (part == 0 && cg == 0)
-            for (uint32_t i = tid; i < a.G * HD; i += 256)
-                for (uint32_t row = 0; row < r.n; ++row)
-                    a.out[(r.first + static_cast<uint64_t>(row)) * a.out_stride + g * a.G * HD + i] = r.bad ? __builtin_nanf("") : 0.0f;
-        return;
+    const bool alone = j_begin == 0 && j_end == tiles.n;
+    const uint32_t lc = lane & 15, lg = lane >> 4;
+    // ---- tiles
+    bool ok = true;
+    const PagedConst<int32_t> table = paged_const(c.table + static_cast<uint64_t>(s) * c.max_pages);
+    const uint32_t in_page = (1u << c.page_log2) - 1;
+    auto tile_of = [&](uint32_t j) { return (j < tiles.sinks ? j : tiles.main + (j - tiles.sinks)) * POS; };
+    // a lane's first bytes of a 16-position block of keys, of values
+    const uint32_t k_lane = (lc * HD + lg * (16 / sizeof(KV))) * sizeof(KV), v_lane = (4 * lg * HD + lc * (HALF ? HD / 16 : 4)) * sizeof(KV);
+    // a row that some column sees
+    auto live = [&](uint32_t t) { return t <= tiles.P_hi && (t >= tiles.start_lo || t < tiles.sink_hi); };
+    auto whole = [&](uint32_t t0) { return (t0 >= tiles.start_hi && t0 + (POS - 1) <= tiles.P_lo) || t0 + (POS - 1) < tiles.sink_lo; };
+    Tile f;
+    uint64_t at[SUB];   // elements of the tile's blocks of 16 positions
+    auto find = [&](uint32_t j) __attribute__((always_inline)) {
+        const uint32_t t0 = tile_of(j);
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const uint32_t lo = t0 + 16 * u;
+            uint32_t page = 0;
+            if (lo <= tiles.P_hi && (lo + 15 >= tiles.start_lo || lo < tiles.sink_hi)) {
+                page = static_cast<uint32_t>(table[lo >> c.page_log2]);
+                if (page >= c.n_pages) {
+                    ok = false;
+                    page = 0;
+                }
+            }
+            at[u] = page * c.page_stride + g * c.head_stride + static_cast<uint64_t>(lo & in_page) * HD;
+        }
+    };
+    auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const uint8_t* const base = reinterpret_cast<const uint8_t*>(kp + at[u]) + k_lane;
+#pragma unroll
+            for (int st = 0; st < KS; ++st) f.k[u][st] = *reinterpret_cast<const std::remove_reference_t<decltype(f.k[u][st])>*>(base + 64 * st);
+        }
+    };
+    auto load_v = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const uint8_t* const base = reinterpret_cast<const uint8_t*>(vp + at[u]) + v_lane;
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                if constexpr (!HALF) {
+#pragma unroll
+                    for (int h = 0; h < Tile::VW; ++h) f.v[p][h] = *reinterpret_cast<const float4*>(base + p * HD * 4 + 256 * h);
+                } else if constexpr (HD == 128) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(base + p * HD * 2);
+                    f.v[4 * u + p][0] = x.x; f.v[4 * u + p][1] = x.y; f.v[4 * u + p][2] = x.z; f.v[4 * u + p][3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(base + p * HD * 2);
+                    f.v[4 * u + p][0] = x.x; f.v[4 * u + p][1] = x.y;
+                }
+            }
+        }
+    };
+    // The decode step's own row is not in its page yet: lanes that hold a piece of it take that from the new rows, narrowed as the
+    // cache's.
+    const uint64_t own = r.first * a.kv_stride + g * HD;
+    auto own_key = [&](uint32_t t0) __attribute__((always_inline)) {
+        const float* const kn = a.k_new + own + lg * (16 / sizeof(KV));
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
+            if (t0 + 16 * u + lc == tiles.P_hi) {
+#pragma unroll
+                for (int st = 0; st < KS; ++st) {
+                    if constexpr (HALF) {
+                        const float4 y = *reinterpret_cast<const float4*>(kn + 32 * st), z = *reinterpret_cast<const float4*>(kn + 32 * st + 4);
+                        f.k[u][st] = make_uint4(f2h(y.x) | f2h(y.y) << 16, f2h(y.z) | f2h(y.w) << 16, f2h(z.x) | f2h(z.y) << 16, f2h(z.z) | f2h(z.w) << 16);
+                    } else {
+                        f.k[u][st] = *reinterpret_cast<const float4*>(kn + 16 * st);
+                    }
+                }
+            }
+    };
+    auto own_value = [&](uint32_t t0) __attribute__((always_inline)) {
+        const float* const vn = a.v_new + own + lc * (HALF ? HD / 16 : 4);
+        const uint32_t p0 = tiles.P_hi - t0;   // the row's place in the tile
+        if (lg == (p0 >> 2 & 3)) {
+#pragma unroll
+            for (int e = 0; e < Tile::VW; ++e) {
+                if constexpr (HALF) {
+                    const float2 y = *reinterpret_cast<const float2*>(vn + 2 * e);
+                    const uint32_t d = f2h(y.x) | f2h(y.y) << 16;
+#pragma unroll
+                    for (int p = 0; p < NS; ++p)
+                        if (static_cast<uint32_t>(p) == ((p0 >> 4) << 2 | (p0 & 3))) f.v[p][e] = d;
+                } else {
+                    const float4 y = *reinterpret_cast<const float4*>(vn + 64 * e);
+#pragma unroll
+                    for (int p = 0; p < NS; ++p)
+                        if (static_cast<uint32_t>(p) == (p0 & 3)) f.v[p][e] = y;
+                }
+            }
+        }
+    };
+
+    // the first tile is on its way while the columns are made ready
+    uint32_t j = j_begin + w;
+    if (j < j_end) {
+        find(j);
+        load_k();
+        load_v();
     }
-    const uint32_t n_cols = r.n * a.G;
-    if (c0 >= n_cols) return;
-    const uint32_t c_last = min(c0 + NC, n_cols) - 1;
-    const PagedTiles tiles = paged_tiles(r, c0, c_last, a);
-    const uint32_t j_end = min((part + 1) * a.part_tiles, tiles.n);   // a part that is all has part_tiles up to 2^31 - 1
-    if (part * a.part_tiles >= tiles.n) return;
-    const bool alone = tiles.n <= a.part_tiles;
 
     // ---- the lane's columns
-    const uint32_t lc = lane & 15, lg = lane >> 4;
     const bool low = HALF && (lc & 8);
     uint32_t P[CB], start[CB], sink[CB], col[CB];
     float mul[CB];
@@ -153,54 +257,6 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
         }
     }
 
-    // ---- tiles
-    bool ok = true;
-    const int32_t* const table = c.table + static_cast<uint64_t>(s) * c.max_pages;
-    const uint32_t in_page = (1u << c.page_log2) - 1;
-    auto tile_of = [&](uint32_t j) { return (j < tiles.sinks ? j : tiles.main + (j - tiles.sinks)) * POS; };
-    // a row that some column sees
-    auto live = [&](uint32_t t) { return t <= tiles.P_hi && (t >= tiles.start_lo || t < tiles.sink_hi); };
-    auto whole = [&](uint32_t t0) { return (t0 >= tiles.start_hi && t0 + (POS - 1) <= tiles.P_lo) || t0 + (POS - 1) < tiles.sink_lo; };
-    auto load = [&](Tile& f, uint32_t j) __attribute__((always_inline)) {
-        const uint32_t t0 = tile_of(j);
-        uint64_t at[SUB];
-#pragma unroll
-        for (int u = 0; u < SUB; ++u) {
-            const uint32_t lo = t0 + 16 * u;
-            uint32_t page = 0;
-            if (lo <= tiles.P_hi && (lo + 15 >= tiles.start_lo || lo < tiles.sink_hi)) {
-                page = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(table[lo >> c.page_log2]));
-                if (page >= c.n_pages) {
-                    ok = false;
-                    page = 0;
-                }
-            }
-            at[u] = page * c.page_stride + g * c.head_stride + static_cast<uint64_t>(lo & in_page) * HD;
-        }
-#pragma unroll
-        for (int u = 0; u < SUB; ++u)
-#pragma unroll
-            for (int st = 0; st < KS; ++st) f.k[u][st] = *reinterpret_cast<const std::remove_reference_t<decltype(f.k[u][st])>*>(kp + at[u] + lc * HD + (lg + 4 * st) * (16 / sizeof(KV)));
-        if constexpr (HALF) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                const KV* const row = vp + at[p >> 2] + (4 * lg + (p & 3)) * HD + lc * (HD / 16);
-                if constexpr (HD == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(row);
-                    f.v[p][0] = x.x; f.v[p][1] = x.y; f.v[p][2] = x.z; f.v[p][3] = x.w;
-                } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(row);
-                    f.v[p][0] = x.x; f.v[p][1] = x.y;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-#pragma unroll
-                for (int h = 0; h < Tile::VW; ++h) f.v[p][h] = *reinterpret_cast<const float4*>(vp + at[0] + (4 * lg + p) * HD + 64 * h + 4 * lc);
-        }
-    };
-
     float m[CB], l[CB];
     paged_f4 o[CB][NO];
 #pragma unroll
@@ -211,27 +267,17 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
         for (int i = 0; i < NO; ++i) o[b][i] = paged_f4{0.f, 0.f, 0.f, 0.f};
     }
 
-    auto compute = [&](Tile& f, uint32_t j) __attribute__((always_inline)) {
+    for (; j < j_end; j += 4) {
         const uint32_t t0 = tile_of(j);
         const bool edge = !whole(t0);
-        if (edge) {   // what no column sees may hold anything, and 0 times that is not 0
-#pragma unroll
-            for (int p = 0; p < NS; ++p)
-                if (!live(t0 + 16 * (p >> 2) + 4 * lg + (p & 3))) {
-                    if constexpr (HALF) {
-#pragma unroll
-                        for (int e = 0; e < Tile::VW; ++e) f.v[p][e] = 0;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < Tile::VW; ++e) f.v[p][e] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                }
-        }
+        const bool newest = a.k_new && t0 + POS > tiles.P_hi, more = j + 4 < j_end;
+        if (newest) own_key(t0);
+        if (more) find(j + 4);
         uint4 ph[HALF ? CB : 1];
         float pf[HALF ? 1 : CB][4];
+        float x[CB][NS];
 #pragma unroll
         for (int b = 0; b < CB; ++b) {
-            float x[NS];
 #pragma unroll
             for (int u = 0; u < SUB; ++u) {
                 paged_f4 d = {0.f, 0.f, 0.f, 0.f};
@@ -251,25 +297,31 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
                     }
                 }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[4 * u + e] = d[e] * mul[b];
+                for (int e = 0; e < 4; ++e) x[b][4 * u + e] = d[e] * mul[b];
             }
+        }
+        // the next tile's keys are on their way while this one's weights are made, its values while the next one's scores are
+        if (more) load_k();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < CB; ++b) {
             if (edge) {
 #pragma unroll
                 for (int p = 0; p < NS; ++p) {
                     const uint32_t t = t0 + 16 * (p >> 2) + 4 * lg + (p & 3);
-                    if (!(t < sink[b] || (t >= start[b] && t <= P[b]))) x[p] = -__builtin_inff();
+                    if (!(t < sink[b] || (t >= start[b] && t <= P[b]))) x[b][p] = -__builtin_inff();
                 }
             }
             if (MASS) {
                 if (!low && col[b] <= c_last) {
                     float* const to = a.scores + (static_cast<uint64_t>(s) * c.n_kv * a.G + g * a.G + col[b]) * a.score_stride + t0 + 4 * lg;
 #pragma unroll
-                    for (int u = 0; u < SUB; ++u) *reinterpret_cast<float4*>(to + 16 * u) = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+                    for (int u = 0; u < SUB; ++u) *reinterpret_cast<float4*>(to + 16 * u) = make_float4(x[b][4 * u], x[b][4 * u + 1], x[b][4 * u + 2], x[b][4 * u + 3]);
                 }
             }
-            float top = x[0];
+            float top = x[b][0];
 #pragma unroll
-            for (int p = 1; p < NS; ++p) top = fmaxf(top, x[p]);
+            for (int p = 1; p < NS; ++p) top = fmaxf(top, x[b][p]);
             if (__any(top > m[b])) {
                 const float mn = fmaxf(m[b], paged_xor_max(top)), f0 = __builtin_amdgcn_exp2f(m[b] - mn);
                 m[b] = mn;
@@ -280,23 +332,37 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
             const float base = m[b] - PAGED_P_LOG2;
 #pragma unroll
             for (int p = 0; p < NS; ++p) {
-                x[p] = __builtin_amdgcn_exp2f(x[p] - base);
-                l[b] += x[p];
+                x[b][p] = __builtin_amdgcn_exp2f(x[b][p] - base);
+                l[b] += x[b][p];
             }
             if constexpr (HALF) {
                 const uint32_t mask = low ? 0xFFFFE000u : 0u;
                 uint32_t d[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float z0 = x[2 * e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[2 * e]) & mask),
-                                z1 = x[2 * e + 1] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[2 * e + 1]) & mask);
+                    const float z0 = x[b][2 * e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[b][2 * e]) & mask),
+                                z1 = x[b][2 * e + 1] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[b][2 * e + 1]) & mask);
                     d[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(z0, z1));
                 }
                 ph[b] = make_uint4(d[0], d[1], d[2], d[3]);
             } else {
 #pragma unroll
-                for (int p = 0; p < 4; ++p) pf[b][p] = x[p];
+                for (int p = 0; p < 4; ++p) pf[b][p] = x[b][p];
             }
+        }
+        if (newest) own_value(t0);
+        if (edge) {   // what no column sees may hold anything, and 0 times that is not 0
+#pragma unroll
+            for (int p = 0; p < NS; ++p)
+                if (!live(t0 + 16 * (p >> 2) + 4 * lg + (p & 3))) {
+                    if constexpr (HALF) {
+#pragma unroll
+                        for (int e = 0; e < Tile::VW; ++e) f.v[p][e] = 0;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < Tile::VW; ++e) f.v[p][e] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    }
+                }
         }
         // ---- O^T += V^T P^T
         if constexpr (HALF) {
@@ -324,30 +390,18 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
                     }
                 }
         }
-    };
-
-    // the next tile's loads are on their way while one is multiplied, where the registers hold two
-    uint32_t j = part * a.part_tiles + w;
-    Tile fa;
-    if constexpr (CB == 2 && HD == 128) {
-        for (; j < j_end; j += 4) {
-            load(fa, j);
-            compute(fa, j);
-        }
-    } else {
-        Tile fb;
-        if (j < j_end) load(fa, j);
-        while (j < j_end) {
-            if (j + 4 < j_end) load(fb, j + 4);
-            compute(fa, j);
-            j += 4;
-            if (j >= j_end) break;
-            if (j + 4 < j_end) load(fa, j + 4);
-            compute(fb, j);
-            j += 4;
-        }
+        if (more) load_v();
+        __builtin_amdgcn_sched_barrier(0);
     }
 
+    // ---- the new row into its page, by the wavefront that had its tile
+    if (a.k_new && cg == 0 && j_end == tiles.n && (tiles.n - 1 - j_begin) % 4 == w && lane < HD / 2) {
+        bool in = true;
+        const uint32_t page = paged_page(c, s, tiles.P_hi, in), c4 = lane % (HD / 4);
+        if (in)
+            KvOps<KV>::st4((lane < HD / 4 ? kp : vp) + paged_row<HD>(c, page, g, tiles.P_hi), c4,
+                           *reinterpret_cast<const float4*>((lane < HD / 4 ? a.k_new : a.v_new) + r.first * a.kv_stride + g * HD + 4 * c4));
+    }
     // ---- the four wavefronts joined
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
@@ -355,15 +409,15 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
         if (!ok) l[b] = __builtin_nanf("");
         const uint32_t lcol = b * CW + (HALF ? lc & 7 : lc);
         if (lg == 0 && !low) {
-            s_m[w][lcol] = m[b];
-            s_l[w][lcol] = l[b];
+            sh.m[w][lcol] = m[b];
+            sh.l[w][lcol] = l[b];
         }
     }
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
         const uint32_t lcol = b * CW + (HALF ? lc & 7 : lc);
-        const float M = fmaxf(fmaxf(s_m[0][lcol], s_m[1][lcol]), fmaxf(s_m[2][lcol], s_m[3][lcol])), f0 = __builtin_amdgcn_exp2f(m[b] - M);
+        const float M = fmaxf(fmaxf(sh.m[0][lcol], sh.m[1][lcol]), fmaxf(sh.m[2][lcol], sh.m[3][lcol])), f0 = __builtin_amdgcn_exp2f(m[b] - M);
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll
@@ -371,32 +425,115 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, const K
                 float x = o[b][i][e];
                 if constexpr (HALF) x += dpp_f<0x128>(x);
                 const uint32_t d = HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3);
-                if (!low) s_o[w][lcol][d] = x * f0;
+                if (!low) sh.o[w][lcol][d] = x * f0;
             }
     }
     __syncthreads();
-    const uint64_t item = (static_cast<uint64_t>(s) * gridDim.x + blockIdx.x) * a.max_parts + part;
+    const uint32_t gx = g * a.n_cg + cg;
+    const uint64_t item = static_cast<uint64_t>(gx) * 2 * a.spans + slot;
     for (uint32_t i = tid; i < NC * (HD / 4); i += 256) {
         const uint32_t lcol = i / (HD / 4), d = i % (HD / 4) * 4, cc = c0 + lcol;
         if (cc > c_last) continue;
-        const float M = fmaxf(fmaxf(s_m[0][lcol], s_m[1][lcol]), fmaxf(s_m[2][lcol], s_m[3][lcol]));
+        const float M = fmaxf(fmaxf(sh.m[0][lcol], sh.m[1][lcol]), fmaxf(sh.m[2][lcol], sh.m[3][lcol]));
         float L = 0.0f;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            L = fmaf(__builtin_amdgcn_exp2f(s_m[u][lcol] - M), s_l[u][lcol], L);
-            const float4 y = *reinterpret_cast<const float4*>(&s_o[u][lcol][d]);
+            L = fmaf(__builtin_amdgcn_exp2f(sh.m[u][lcol] - M), sh.l[u][lcol], L);
+            const float4 y = *reinterpret_cast<const float4*>(&sh.o[u][lcol][d]);
             x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         if (alone) {
             const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             *reinterpret_cast<float4*>(a.out + (r.first + static_cast<uint64_t>(cc / a.G)) * a.out_stride + (g * a.G + cc % a.G) * HD + d) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            if (MASS && d == 0) *reinterpret_cast<float2*>(a.ml_seq + ((static_cast<uint64_t>(gx) * a.n_rows + s) * NC + lcol) * 2) = make_float2(M, L);
         } else {
             *reinterpret_cast<float4*>(a.acc + (item * NC + lcol) * HD + d) = x;
+            if (d == 0) *reinterpret_cast<float2*>(a.ml + (item * NC + lcol) * 2) = make_float2(M, L);
         }
-        if ((MASS || !alone) && d == 0) {
-            a.ml[(item * NC + lcol) * 2] = M;
-            a.ml[(item * NC + lcol) * 2 + 1] = L;
+    }
+}
+
+// A kv head and group of columns has one list of tiles, sequence after sequence.  Either a workgroup takes a sequence of it, grid =
+// (kv heads * groups, sequences), or each takes a span of equal length, grid = (kv heads * groups, spans): ragged sequences then cost
+// what their sum costs.  Only the first and the last sequence of a span can be cut: slots 2 span and 2 span + 1.
+template <typename KV, int HD, int CB, bool MASS>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, PagedOp a, uint32_t n_seqs) {
+    constexpr int NC = (sizeof(KV) == 2 ? 8 : 16) * CB;
+    __shared__ PagedShared<NC, HD> sh;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x / a.n_cg, cg = blockIdx.x % a.n_cg, c0 = cg * NC;
+    uint32_t s = blockIdx.y, j = 0, left = 0xFFFFFFFFu, span = 0;   // the sequence, the first of its tiles, tiles left of the span
+    uint32_t s_end = s + 1;
+    if (a.spans) {
+        span = blockIdx.y;
+        s_end = n_seqs;
+        // all tiles, and the sequence that has tile `at`; up to 64 sequences by one look at their lengths
+        uint32_t total = 0, at = 0, share = 0;
+        for (int pass = 0; pass < 2; ++pass) {
+            uint32_t before = 0;
+            bool found = false;
+            for (uint32_t b = 0; b < n_seqs && !found; b += 64) {
+                const uint32_t n = b + lane < n_seqs ? paged_count(c, a, b + lane, c0) : 0;
+                uint32_t inc = n;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t o = __shfl_up(inc, d);
+                    if (lane >= static_cast<uint32_t>(d)) inc += o;
+                }
+                const uint32_t sum = __builtin_amdgcn_readlane(inc, 63);
+                if (pass == 0) total += sum;
+                if (pass == 0 && n_seqs <= 64) {
+                    share = max(a.least, (total + a.spans - 1) / a.spans);
+                    at = span * share;
+                    pass = 1;
+                }
+                if (pass == 1) {
+                    const uint64_t over = __ballot(before + inc > at);
+                    if (over) {
+                        const int x = __builtin_ctzll(over);
+                        s = b + x;
+                        j = at - before - __builtin_amdgcn_readlane(inc - n, x);
+                        found = true;
+                    }
+                }
+                before += sum;
+            }
+            if (pass == 0) {
+                share = max(a.least, (total + a.spans - 1) / a.spans);
+                at = span * share;
+            }
+        }
+        if (at >= total) return;
+        left = min(share, total - at);
+        s = __builtin_amdgcn_readfirstlane(s);
+        j = __builtin_amdgcn_readfirstlane(j);
+    }
+    for (; s < s_end && left; ++s, j = 0) {
+        const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
+        if (r.bad || r.len == 0) {
+            // nothing is known of these rows but where they are
+            if (cg == 0) {
+                for (uint32_t row = 0; row < r.n; ++row)
+                    for (uint32_t i = tid; i < a.G * HD; i += 256)
+                        a.out[(r.first + static_cast<uint64_t>(row)) * a.out_stride + g * a.G * HD + i] = r.bad ? __builtin_nanf("") : 0.0f;
+                --left;
+            }
+            continue;
+        }
+        const uint32_t n_cols = r.n * a.G;
+        if (c0 >= n_cols) continue;
+        const uint32_t c_last = min(c0 + NC, n_cols) - 1;
+        const PagedTiles tiles = paged_tiles(r, c0, c_last, a);
+        const uint32_t j_end = left < tiles.n - j ? j + left : tiles.n;
+        paged_attn_part<KV, HD, CB, MASS>(sh, c, kp, vp, a, g, cg, s, r, tiles, c0, c_last, j, j_end, 2 * span + (j == 0));
+        if (a.spans) {
+            if (tid == 0) {
+                // the first part says who has the first, the last who has the last
+                uint32_t* const cut = reinterpret_cast<uint32_t*>(a.cut + static_cast<uint64_t>(blockIdx.x) * n_seqs + s);
+                if (j == 0) cut[0] = span;
+                if (j_end == tiles.n) cut[1] = span;
+            }
+            left -= j_end - j;
+            __syncthreads();   // the shared memory again
         }
     }
 }

@@ -95,17 +95,19 @@ struct PagedRows {
     uint32_t len;        // positions of the sequence; row first + i is at position len - n + i
     bool bad;            // lengths or rows out of order: [first, first + n) get NaN, nothing else is touched
 };
-PAGED_HD PagedRows paged_rows(const uint32_t* q_first, const uint32_t* lens, uint32_t s, uint32_t n_rows, uint32_t max_queries, uint32_t max_len) {
+// one row a sequence, and rows [a, b)
+PAGED_HD PagedRows paged_one_row(uint32_t s, uint32_t len, uint32_t max_len) {
     PagedRows r;
-    r.len = lens[s];
-    if (!q_first) {
-        r.first = s;
-        r.n = 1;
-        r.bad = r.len > max_len;
-        return r;
-    }
-    const uint32_t a = q_first[s], b = q_first[s + 1];
-    r.bad = a > b || b > n_rows || b - a > max_queries || b - a > r.len || r.len > max_len;
+    r.len = len;
+    r.first = s;
+    r.n = 1;
+    r.bad = len > max_len;
+    return r;
+}
+PAGED_HD PagedRows paged_chunk_rows(uint32_t a, uint32_t b, uint32_t len, uint32_t n_rows, uint32_t max_queries, uint32_t max_len) {
+    PagedRows r;
+    r.len = len;
+    r.bad = a > b || b > n_rows || b - a > max_queries || b - a > len || len > max_len;
     r.first = a < n_rows ? a : n_rows;
     const uint32_t end = b < n_rows ? b : n_rows;
     r.n = end > r.first ? end - r.first : 0;
@@ -123,22 +125,18 @@ PAGED_HD PagedSeen paged_seen(uint32_t P, uint32_t window, uint32_t n_sink) {
     return v;
 }
 
-// How a sequence's tiles are cut into parts, a workgroup each.  groups: workgroups of a part over all sequences.
+// How the tiles of a kv head and group of columns are cut among workgroups.  wide: kv heads times groups.
 struct PagedCut {
-    uint32_t part_tiles, max_parts;
+    uint32_t spans;   // workgroups, of equal numbers of tiles; 0: one for each sequence
+    uint32_t least;   // tiles of a workgroup at least
 };
-inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint64_t groups, uint32_t n_cu) {
+inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, uint32_t n_cu) {
     // tiles that a sequence of max_len may have: those of the window and of the first positions each touch one more at their ends
     uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
     if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
-    most = std::max<uint64_t>(most, 1);
-    // enough workgroups for four a CU, of at least two tiles a wavefront and at most 1024 positions
-    const uint64_t want = std::max<uint64_t>(1, 4ull * n_cu / std::max<uint64_t>(groups, 1));
-    uint64_t tiles = std::max<uint64_t>(8, (most + want - 1) / want);
-    tiles = std::min<uint64_t>((tiles + 3) / 4 * 4, std::max<uint64_t>(1024 / tile, 8));
-    tiles = std::max<uint64_t>(tiles, ((most + 1023) / 1024 + 3) / 4 * 4);   // and at most 1024 of them
     PagedCut c;
-    c.part_tiles = static_cast<uint32_t>(tiles);
-    c.max_parts = static_cast<uint32_t>((most + tiles - 1) / tiles);
+    c.least = 256 / tile;
+    // two workgroups a CU; short sequences, and groups of columns that fill the chip by themselves, are not cut
+    c.spans = most <= 384 / tile || n_cu < wide ? 0 : 2 * n_cu / wide;
     return c;
 }

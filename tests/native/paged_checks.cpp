@@ -100,11 +100,11 @@ int main() {
     struct Want { uint32_t first, n; bool bad; };
     const Want want[5] = {{3, 0, true}, {1, 7, true}, {8, 3, false}, {11, 9, true}, {20, 0, true}};
     for (uint32_t s = 0; s < 5; ++s) {
-        const PagedRows r = paged_rows(f, n, s, 20, 6, 64);
+        const PagedRows r = paged_chunk_rows(f[s], f[s + 1], n[s], 20, 6, 64);
         expect(r.first == want[s].first && r.n == want[s].n && r.bad == want[s].bad, "rows of a sequence");
         expect(static_cast<uint64_t>(r.first) + r.n <= 20, "rows stay in bounds");
     }
-    expect(paged_rows(nullptr, n, 0, 5, 1, 39).bad && !paged_rows(nullptr, n, 4, 5, 1, 39).bad, "lengths of the decode form");
+    expect(paged_one_row(0, n[0], 39).bad && !paged_one_row(4, n[4], 39).bad, "lengths of the decode form");
     // what a row sees, against the definition
     for (uint32_t P = 0; P < 40; ++P)
         for (uint32_t w : {0u, 1u, 7u, 16u, 39u, 40u, 100u, 0xFFFFFFFFu})
