@@ -3,6 +3,7 @@
 
 #include "paged.hip.h"
 #include "paged_attn.hip.h"
+#include "paged_chunk.hip.h"
 
 // ---- chunks: the new rows into their pages -----------------------------------------------------------------------------
 // grid = (blocks, sequences); a thread moves four floats of a row's keys and values
@@ -24,6 +25,106 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __re
         const uint64_t dst = paged_row<HD>(c, page, g, t), src = (r.first + static_cast<uint64_t>(row)) * kv_stride + g * HD;
         KvOps<KV>::st4(kp + dst, c4, *reinterpret_cast<const float4*>(k_new + src + 4 * c4));
         KvOps<KV>::st4(vp + dst, c4, *reinterpret_cast<const float4*>(v_new + src + 4 * c4));
+    }
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------
+template <typename KV_, int HD, int CB, bool MASS> struct PagedFew {
+    using KV = KV_;
+    static constexpr int NC = (sizeof(KV) == 2 ? 8 : 16) * CB, DIM = HD;
+    using Shared = PagedShared<NC, HD>;
+    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_attn_part<KV, HD, CB, MASS>(sh, x...); }
+};
+template <int HD> struct PagedMany {
+    using KV = kv_half;
+    static constexpr int NC = 128, DIM = HD;
+    using Shared = PagedChunkShared<HD>;
+    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_chunk_part<HD>(sh, x...); }
+};
+
+// A kv head and group of columns has one list of tiles, sequence after sequence.  Either a workgroup takes a sequence of it, grid =
+// (kv heads * groups, sequences), or each takes a span of equal length, grid = (kv heads * groups, spans): ragged sequences then cost
+// what their sum costs.  Only the first and the last sequence of a span can be cut: slots 2 span and 2 span + 1.
+// Work: PagedFew or PagedMany below.
+template <class Work>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typename Work::KV* __restrict__ kp, typename Work::KV* __restrict__ vp, PagedOp a, uint32_t n_seqs) {
+    constexpr int NC = Work::NC;
+    __shared__ typename Work::Shared sh;
+    // kv heads side by side, so that a head's workgroups share an XCD's L2 where there are eight; the columns with the most positions first
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x % c.n_kv, cg = a.n_cg - 1 - blockIdx.x / c.n_kv, c0 = cg * NC;
+    uint32_t s = blockIdx.y, j = 0, left = 0xFFFFFFFFu, span = 0;   // the sequence, the first of its tiles, tiles left of the span
+    uint32_t s_end = s + 1;
+    if (a.spans) {
+        span = blockIdx.y;
+        s_end = n_seqs;
+        // all tiles, and the sequence that has tile `at`; up to 64 sequences by one look at their lengths
+        uint32_t total = 0, at = 0, share = 0;
+        for (int pass = 0; pass < 2; ++pass) {
+            uint32_t before = 0;
+            bool found = false;
+            for (uint32_t b = 0; b < n_seqs && !found; b += 64) {
+                const uint32_t n = b + lane < n_seqs ? paged_count(c, a, b + lane, c0) : 0;
+                uint32_t inc = n;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const uint32_t o = __shfl_up(inc, d);
+                    if (lane >= static_cast<uint32_t>(d)) inc += o;
+                }
+                const uint32_t sum = __builtin_amdgcn_readlane(inc, 63);
+                if (pass == 0) total += sum;
+                if (pass == 0 && n_seqs <= 64) {
+                    share = max(a.least, (total + a.spans - 1) / a.spans);
+                    at = span * share;
+                    pass = 1;
+                }
+                if (pass == 1) {
+                    const uint64_t over = __ballot(before + inc > at);
+                    if (over) {
+                        const int x = __builtin_ctzll(over);
+                        s = b + x;
+                        j = at - before - __builtin_amdgcn_readlane(inc - n, x);
+                        found = true;
+                    }
+                }
+                before += sum;
+            }
+            if (pass == 0) {
+                share = max(a.least, (total + a.spans - 1) / a.spans);
+                at = span * share;
+            }
+        }
+        if (at >= total) return;
+        left = min(share, total - at);
+        s = __builtin_amdgcn_readfirstlane(s);
+        j = __builtin_amdgcn_readfirstlane(j);
+    }
+    for (; s < s_end && left; ++s, j = 0) {
+        const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
+        if (r.bad || r.len == 0) {
+            // nothing is known of these rows but where they are
+            if (cg == 0) {
+                for (uint32_t row = 0; row < r.n; ++row)
+                    for (uint32_t i = tid; i < a.G * Work::DIM; i += 256)
+                        a.out[(r.first + static_cast<uint64_t>(row)) * a.out_stride + g * a.G * Work::DIM + i] = r.bad ? __builtin_nanf("") : 0.0f;
+                --left;
+            }
+            continue;
+        }
+        const uint32_t n_cols = r.n * a.G;
+        if (c0 >= n_cols) continue;
+        const uint32_t c_last = min(c0 + NC, n_cols) - 1;
+        const PagedTiles tiles = paged_tiles(r, c0, c_last, a);
+        const uint32_t j_end = left < tiles.n - j ? j + left : tiles.n;
+        Work::part(sh, c, kp, vp, a, g, cg, s, r, tiles, c0, c_last, j, j_end, 2 * span + (j == 0));
+        if (a.spans) {
+            if (tid == 0) {
+                // the first part says who has the first, the last who has the last
+                uint32_t* const cut = reinterpret_cast<uint32_t*>(a.cut + static_cast<uint64_t>(g * a.n_cg + cg) * n_seqs + s);
+                if (j == 0) cut[0] = span;
+                if (j_end == tiles.n) cut[1] = span;
+            }
+            left -= j_end - j;
+            __syncthreads();   // the shared memory again
+        }
     }
 }
 
@@ -146,8 +247,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.scale2 = in.scale * 1.44269504088896340736f;
     a.window = in.window; a.n_sink = in.n_sink;
     const uint64_t cols = static_cast<uint64_t>(a.max_queries) * a.G;
+    const bool many = HALF && in.q_first && cols > 48;
     const uint32_t cb = HALF && cols > 8 ? 2 : 1;
-    a.n_cols = (HALF ? 8 : 16) * cb;
+    a.n_cols = many ? 128 : (HALF ? 8 : 16) * cb;
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
     if (static_cast<uint64_t>(c.n_kv_heads) * a.n_cg > (1u << 23)) return cera_fail(ctx, CERA_HIP_ERR_SHAPE, "paged attention: too many rows of a sequence for one call");
     a.tile = HALF ? 32 : 16;
@@ -181,22 +283,23 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     }
     const dim3 grid(wide, a.spans ? a.spans : c.n_seqs);
     auto launch = [&](auto tag) {
-        constexpr int CB = decltype(tag)::value;
-        if (a.mass) hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, true>), grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
-        else hipLaunchKernelGGL((paged_attn_kernel<KV, HD, CB, false>), grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
+        using Work = decltype(tag);
+        hipLaunchKernelGGL(paged_attn_kernel<Work>, grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
     };
-    if (cb == 2) {
-        if constexpr (HALF) launch(std::integral_constant<int, 2>{});
+    if constexpr (HALF) {
+        if (many) launch(PagedMany<HD>{});
+        else if (cb == 2) { if (a.mass) launch(PagedFew<KV, HD, 2, true>{}); else launch(PagedFew<KV, HD, 2, false>{}); }
+        else { if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{}); }
     } else {
-        launch(std::integral_constant<int, 1>{});
+        if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{});
     }
     if (a.spans || a.mass) {
-        const bool many = a.spans > 8;   // parts of a column shared out
-        const uint32_t cols_wg = 256 / (HD / 4 * (many ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
+        const bool shared = a.spans > 8;   // parts of a column shared out
+        const uint32_t cols_wg = 256 / (HD / 4 * (shared ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
         const uint32_t mass = a.mass ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;
         const dim3 blocks(merge + mass * c.n_kv_heads, c.n_seqs);
-        if (many) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
+        if (shared) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
         else hipLaunchKernelGGL((paged_finish_kernel<HD, 1>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
     }
     HIP_TRY(ctx, hipGetLastError());

@@ -453,87 +453,3 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
         }
     }
 }
-
-// A kv head and group of columns has one list of tiles, sequence after sequence.  Either a workgroup takes a sequence of it, grid =
-// (kv heads * groups, sequences), or each takes a span of equal length, grid = (kv heads * groups, spans): ragged sequences then cost
-// what their sum costs.  Only the first and the last sequence of a span can be cut: slots 2 span and 2 span + 1.
-template <typename KV, int HD, int CB, bool MASS>
-__global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, PagedOp a, uint32_t n_seqs) {
-    constexpr int NC = (sizeof(KV) == 2 ? 8 : 16) * CB;
-    __shared__ PagedShared<NC, HD> sh;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x / a.n_cg, cg = blockIdx.x % a.n_cg, c0 = cg * NC;
-    uint32_t s = blockIdx.y, j = 0, left = 0xFFFFFFFFu, span = 0;   // the sequence, the first of its tiles, tiles left of the span
-    uint32_t s_end = s + 1;
-    if (a.spans) {
-        span = blockIdx.y;
-        s_end = n_seqs;
-        // all tiles, and the sequence that has tile `at`; up to 64 sequences by one look at their lengths
-        uint32_t total = 0, at = 0, share = 0;
-        for (int pass = 0; pass < 2; ++pass) {
-            uint32_t before = 0;
-            bool found = false;
-            for (uint32_t b = 0; b < n_seqs && !found; b += 64) {
-                const uint32_t n = b + lane < n_seqs ? paged_count(c, a, b + lane, c0) : 0;
-                uint32_t inc = n;
-                for (int d = 1; d < 64; d <<= 1) {
-                    const uint32_t o = __shfl_up(inc, d);
-                    if (lane >= static_cast<uint32_t>(d)) inc += o;
-                }
-                const uint32_t sum = __builtin_amdgcn_readlane(inc, 63);
-                if (pass == 0) total += sum;
-                if (pass == 0 && n_seqs <= 64) {
-                    share = max(a.least, (total + a.spans - 1) / a.spans);
-                    at = span * share;
-                    pass = 1;
-                }
-                if (pass == 1) {
-                    const uint64_t over = __ballot(before + inc > at);
-                    if (over) {
-                        const int x = __builtin_ctzll(over);
-                        s = b + x;
-                        j = at - before - __builtin_amdgcn_readlane(inc - n, x);
-                        found = true;
-                    }
-                }
-                before += sum;
-            }
-            if (pass == 0) {
-                share = max(a.least, (total + a.spans - 1) / a.spans);
-                at = span * share;
-            }
-        }
-        if (at >= total) return;
-        left = min(share, total - at);
-        s = __builtin_amdgcn_readfirstlane(s);
-        j = __builtin_amdgcn_readfirstlane(j);
-    }
-    for (; s < s_end && left; ++s, j = 0) {
-        const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
-        if (r.bad || r.len == 0) {
-            // nothing is known of these rows but where they are
-            if (cg == 0) {
-                for (uint32_t row = 0; row < r.n; ++row)
-                    for (uint32_t i = tid; i < a.G * HD; i += 256)
-                        a.out[(r.first + static_cast<uint64_t>(row)) * a.out_stride + g * a.G * HD + i] = r.bad ? __builtin_nanf("") : 0.0f;
-                --left;
-            }
-            continue;
-        }
-        const uint32_t n_cols = r.n * a.G;
-        if (c0 >= n_cols) continue;
-        const uint32_t c_last = min(c0 + NC, n_cols) - 1;
-        const PagedTiles tiles = paged_tiles(r, c0, c_last, a);
-        const uint32_t j_end = left < tiles.n - j ? j + left : tiles.n;
-        paged_attn_part<KV, HD, CB, MASS>(sh, c, kp, vp, a, g, cg, s, r, tiles, c0, c_last, j, j_end, 2 * span + (j == 0));
-        if (a.spans) {
-            if (tid == 0) {
-                // the first part says who has the first, the last who has the last
-                uint32_t* const cut = reinterpret_cast<uint32_t*>(a.cut + static_cast<uint64_t>(blockIdx.x) * n_seqs + s);
-                if (j == 0) cut[0] = span;
-                if (j_end == tiles.n) cut[1] = span;
-            }
-            left -= j_end - j;
-            __syncthreads();   // the shared memory again
-        }
-    }
-}

@@ -1,0 +1,223 @@
+// Attention of many (row, query head) columns of a kv head over a paged half cache: chunks of new tokens.
+//
+// The products are those of paged_attn.hip.h in 32 x 32 x 16 form, S^T = K Q^T and O^T = V^T P^T, a wavefront for 32 columns, four of
+// them on the same tiles of 32 positions.  Loads go straight into LDS, the next tile's while this one is multiplied: one barrier a
+// tile.  A row's 16-byte pieces lie at places exchanged by its number, so that neither the keys' reads (a lane per row) nor the
+// values' (transposing reads of 4 rows x 16 dims) meet in a bank; the exchange is made on the way in, by what a lane loads.
+// q and the weights are pairs hi + lo of halves here too, two products each: f32's accuracy at twice the operations.
+// What bounds it are the matrix cores, with the softmax between the products in the shadow of the other wavefronts.
+#pragma once
+#include "lds_dma.hip.h"
+#include "paged_attn.hip.h"
+
+typedef float paged_f16v __attribute__((ext_vector_type(16)));
+typedef short paged_s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) paged_s4* paged_lds4;
+
+template <int HD> struct PagedChunkShared {
+    __attribute__((aligned(1024))) uint8_t tile[2][2][32 * HD * 2];   // [buffer][keys, values]
+    uint32_t bad;
+};
+
+// place of 16-byte piece `piece` in row `row` of a tile
+template <int HD, bool VALUES> __device__ __forceinline__ uint32_t paged_piece(uint32_t row, uint32_t piece) {
+    if constexpr (HD == 128) return piece ^ (VALUES ? (row & 3) << 2 : row & 15);
+    else return piece ^ (VALUES ? (row >> 1 & 1) << 2 : row >> 1 & 7);
+}
+
+// Tiles [j_begin, j_end) of sequence s for 128 columns from c0 on; slot: of a part's results.
+template <int HD>
+__device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const PagedView& c, const kv_half* __restrict__ kp, const kv_half* __restrict__ vp, const PagedOp& a, uint32_t g,
+                                                 uint32_t cg, uint32_t s, const PagedRows& r, const PagedTiles& tiles, uint32_t c0, uint32_t c_last, uint32_t j_begin, uint32_t j_end,
+                                                 uint32_t slot) {
+    constexpr int KS = HD / 16, ND = HD / 32;            // steps over the dims, 32-row tiles of O^T
+    constexpr uint32_t ROW = HD * 2, PIECES = HD / 8;    // bytes and 16-byte pieces of a row
+    constexpr uint32_t ROWS_KB = 1024 / ROW;             // rows of one load of a wavefront
+    constexpr int LOADS = 16 / ROWS_KB;                  // loads of a block of 16 positions
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid >> 6)));
+    const uint32_t lc = lane & 31, half = lane >> 5;
+    const bool alone = j_begin == 0 && j_end == tiles.n;
+    const uint32_t in_page = (1u << c.page_log2) - 1;
+    const PagedConst<int32_t> table = paged_const(c.table + static_cast<uint64_t>(s) * c.max_pages);
+    auto tile_of = [&](uint32_t j) { return (j < tiles.sinks ? j : tiles.main + (j - tiles.sinks)) * 32; };
+
+    // ---- loads: a wavefront has one block of 16 positions of the tile's keys or of its values
+    bool ok = true;
+    const uint32_t blk = w & 1;
+    const bool values = w >= 2;
+    const uint8_t* const pool = reinterpret_cast<const uint8_t*>(values ? vp : kp);
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int k = 0; k < LOADS; ++k) {
+        const uint32_t row = k * ROWS_KB + lane / PIECES, at = lane % PIECES;   // of the block; its number in the tile differs by 16, which no exchange looks at
+        off[k] = row * ROW + (values ? paged_piece<HD, true>(row, at) : paged_piece<HD, false>(row, at)) * 16;
+    }
+    const uint32_t dst = lds_addr(sh.tile[0][values]) + blk * 16 * ROW;
+    auto load = [&](uint32_t j, uint32_t buf) __attribute__((always_inline)) {
+        const uint32_t lo = tile_of(j) + 16 * blk;
+        if (lo <= tiles.P_hi && (lo + 15 >= tiles.start_lo || lo < tiles.sink_hi)) {
+            uint32_t page = static_cast<uint32_t>(table[lo >> c.page_log2]);
+            if (page >= c.n_pages) {
+                ok = false;
+                page = 0;
+            }
+            const uint8_t* const src = lds_dma_base(pool + (page * c.page_stride + g * c.head_stride + static_cast<uint64_t>(lo & in_page) * HD) * 2);
+#pragma unroll
+            for (int k = 0; k < LOADS; ++k) lds_dma_1k(src, off[k], dst + buf * (2 * 32 * ROW) + k * 1024);
+        }
+    };
+    if (tid == 0) sh.bad = 0;
+    uint32_t j = j_begin, buf = 0;
+    load(j, 0);
+
+    // ---- the lane's column
+    const uint32_t w0 = c0 + 32 * w, col = w0 + lc, cc = min(col, c_last), qi = cc / a.G, h = g * a.G + cc % a.G;
+    const uint32_t P = r.len - r.n + qi;
+    const PagedSeen seen = paged_seen(P, a.window, a.n_sink);
+    // of the wavefront's first and last column
+    const uint32_t P_lo = r.len - r.n + min(w0, c_last) / a.G, P_hi = r.len - r.n + min(w0 + 31, c_last) / a.G;
+    const PagedSeen seen_lo = paged_seen(P_lo, a.window, a.n_sink), seen_hi = paged_seen(P_hi, a.window, a.n_sink);
+    const bool idle = w0 > c_last;
+    uint4 qh[KS], ql[KS];
+    float mul;
+    {
+        const float* const qp = a.q + (r.first + static_cast<uint64_t>(qi)) * a.q_stride + h * HD + 8 * half;
+        float top = 0.0f;
+#pragma unroll
+        for (int st = 0; st < KS; ++st)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float4 u = *reinterpret_cast<const float4*>(qp + 16 * st + 4 * e);
+                top = fmaxf(fmaxf(fmaxf(top, fabsf(u.x)), fmaxf(fabsf(u.y), fabsf(u.z))), fabsf(u.w));
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
+        up = min(up, 100);
+        mul = ldexpf(fabsf(a.scale2), -up);
+        const float sign = a.scale2 < 0.0f ? -1.0f : 1.0f;   // so that the largest product is the largest score
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 u = *reinterpret_cast<const float2*>(qp + 16 * st + 2 * e);
+                const float y0 = ldexpf(u.x * sign, up), y1 = ldexpf(u.y * sign, up);
+                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0 - h2f(hi[e] & 0xFFFF), y1 - h2f(hi[e] >> 16)));
+            }
+            qh[st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            ql[st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+    }
+    float m = PAGED_LOWEST, base = -1e30f, l = 0.0f;   // largest product; its score less the weights' exponent; sum of weights
+    paged_f16v o[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+
+    // where a lane reads: keys by row lc, pieces 2 st + half; values by rows 4 half + (lane & 15) / 4, dims 16 (lane / 16 & 1) + 4 (lane & 3)
+    const uint32_t v_row = 4 * half + (lane >> 2 & 3), v_piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), v_byte = 8 * (lane & 1);
+
+    for (; j < j_end; ++j, buf ^= 1) {
+        // this tile is in, and every wavefront is past its reads of the other buffer
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const uint32_t t0 = tile_of(j);
+        if (t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
+            // values that no column sees may be anything, and 0 times that is not 0
+            for (uint32_t i = tid; i < 32 * PIECES; i += 256) {
+                const uint32_t t = t0 + i / PIECES;
+                if (!(t <= tiles.P_hi && (t >= tiles.start_lo || t < tiles.sink_hi))) *reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            __syncthreads();
+        }
+        if (j + 1 < j_end) load(j + 1, buf ^ 1);
+        if (idle || t0 > P_hi || (t0 + 31 < seen_lo.start && t0 >= seen_hi.sink_end)) continue;
+        const uint8_t *const kt = sh.tile[buf][0], *const vt = sh.tile[buf][1];
+        paged_f16v x;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) {
+            const paged_h8 k = __builtin_bit_cast(paged_h8, *reinterpret_cast<const uint4*>(kt + lc * ROW + paged_piece<HD, false>(lc, 2 * st + half) * 16));
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(paged_h8, qh[st]), x, 0, 0, 0);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(paged_h8, ql[st]), x, 0, 0, 0);
+        }
+        // product e is of position t0 + 8 (e / 4) + 4 half + e % 4
+        const bool edge = !((t0 >= seen_hi.start && t0 + 31 <= P_lo) || t0 + 31 < seen_lo.sink_end);
+        uint32_t out_of_sight = 0;
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t t = t0 + 8 * (e >> 2) + 4 * half + (e & 3);
+                if (!(t < seen.sink_end || (t >= seen.start && t <= P))) {
+                    x[e] = -__builtin_inff();
+                    out_of_sight |= 1u << e;
+                }
+            }
+        }
+        float top = x[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
+        if (__any(top > m)) {
+            m = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
+            const float b = m == PAGED_LOWEST ? base : fmaf(m, mul, -PAGED_P_LOG2), f0 = __builtin_amdgcn_exp2f(base - b);
+            base = b;
+            l *= f0;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) o[i] *= f0;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], mul, -base));
+        if (edge) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[e] = out_of_sight >> e & 1 ? 0.0f : x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) l += x[e];
+        uint4 ph[2], pl[2];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float y0 = x[8 * kk + 2 * e], y1 = x[8 * kk + 2 * e + 1];
+                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y0) & 0xFFFFE000u),
+                                                                                 y1 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y1) & 0xFFFFE000u)));
+            }
+            ph[kk] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            pl[kk] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {
+                // slot e of a half is position 16 kk + 8 (e / 4) + 4 half + e % 4
+                paged_s4 v[2];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t row = 16 * kk + 8 * b + v_row;
+                    v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((paged_lds4)(vt + row * ROW + paged_piece<HD, true>(row, 4 * i + v_piece) * 16 + v_byte));
+                }
+                const paged_h8 va = __builtin_bit_cast(paged_h8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, ph[kk]), o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, pl[kk]), o[i], 0, 0, 0);
+            }
+    }
+    l += __shfl_xor(l, 32);
+    if (!ok) sh.bad = 1;
+    __syncthreads();
+    if (sh.bad) l = __builtin_nanf("");
+    if (col > c_last) return;
+    const uint64_t item = (static_cast<uint64_t>(g * a.n_cg + cg) * 2 * a.spans + slot) * a.n_cols + 32 * w + lc;
+    float* const to = alone ? a.out + (r.first + static_cast<uint64_t>(qi)) * a.out_stride + h * HD : a.acc + item * HD;
+    const float inv = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            *reinterpret_cast<float4*>(to + 32 * i + 8 * e + 4 * half) = make_float4(o[i][4 * e] * inv, o[i][4 * e + 1] * inv, o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv);
+    if (!alone && half == 0) *reinterpret_cast<float2*>(a.ml + item * 2) = make_float2(base + PAGED_P_LOG2, l);
+}
