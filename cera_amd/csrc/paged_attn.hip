@@ -51,7 +51,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typenam
     constexpr int NC = Work::NC;
     __shared__ typename Work::Shared sh;
     // kv heads side by side, so that a head's workgroups share an XCD's L2 where there are eight; the columns with the most positions first
-    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x % c.n_kv, cg = a.n_cg - 1 - blockIdx.x / c.n_kv, c0 = cg * NC;
+    // every second round of the chip the other way, so that a CU's add up to about the same
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x % c.n_kv, at_cg = blockIdx.x / c.n_kv, in_round = at_cg % a.round, round0 = at_cg - in_round;
+    const uint32_t cg = a.n_cg - 1 - (round0 / a.round & 1 ? round0 + min(a.round, a.n_cg - round0) - 1 - in_round : at_cg), c0 = cg * NC;
     uint32_t s = blockIdx.y, j = 0, left = 0xFFFFFFFFu, span = 0;   // the sequence, the first of its tiles, tiles left of the span
     uint32_t s_end = s + 1;
     if (a.spans) {
@@ -253,6 +255,7 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
     if (static_cast<uint64_t>(c.n_kv_heads) * a.n_cg > (1u << 23)) return cera_fail(ctx, CERA_HIP_ERR_SHAPE, "paged attention: too many rows of a sequence for one call");
     a.tile = HALF ? 32 : 16;
+    a.round = std::max(1u, ctx->n_cu / c.n_kv_heads);
     const uint32_t wide = c.n_kv_heads * a.n_cg;
     const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, ctx->n_cu);
     a.spans = cut.spans;

@@ -37,6 +37,14 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
     float* const mw = mass + sg * mass_stride;
     // the middle [lo, hi) has more than `need` positions
     const uint32_t lo = n_first, hi = len - n_recent, need = budget - n_first - n_recent;
+    // the first keys stay in registers between the passes
+    constexpr uint32_t HELD = 8;
+    uint32_t held[HELD];
+#pragma unroll
+    for (uint32_t u = 0; u < HELD; ++u) {
+        const uint32_t t = lo + tid + u * EV_THREADS;
+        held[u] = t < hi ? evict_key(mw[t]) : 0;
+    }
     // radix selection: `prefix` holds the bits found so far, `left` how many of those that share them still stay
     uint32_t prefix = 0, left = need;
     if (need) {
@@ -44,10 +52,13 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
             const uint32_t shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, above = shift + bits;
             for (uint32_t b = tid; b < EV_BINS; b += EV_THREADS) hist[b] = 0;
             __syncthreads();
-            for (uint32_t t = lo + tid; t < hi; t += EV_THREADS) {
-                const uint32_t k = evict_key(mw[t]);
+            auto count = [&](uint32_t k) {
                 if (pass == 0 || k >> above == prefix >> above) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)], 1u);
-            }
+            };
+#pragma unroll
+            for (uint32_t u = 0; u < HELD; ++u)
+                if (lo + tid + u * EV_THREADS < hi) count(held[u]);
+            for (uint32_t t = lo + tid + HELD * EV_THREADS; t < hi; t += EV_THREADS) count(evict_key(mw[t]));
             __syncthreads();
             // from the top bin down to the one in which the count reaches `left`: two bins a thread, thread 0 has the highest
             const uint32_t top = (1u << bits) - 1, n_thr = (1u << bits) / 2;
@@ -106,31 +117,57 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
 }
 
 // grid = (128-byte columns of a row, 2 * kv heads, sequences): keys, then values.  Eight lanes of 16 bytes a row.
-static constexpr uint32_t EV_ROWS = 32, EV_UNROLL = 8;   // rows of a workgroup's pass, passes of a step
+// A step's rows are on their way while the ones before are written: sources lie behind all of what is written until then.
+static constexpr uint32_t EV_ROWS = EV_THREADS / 8, EV_UNROLL = 2, EV_STEP = EV_ROWS * EV_UNROLL;   // rows of a pass, passes and rows of a step
 template <typename KV, int HD>
-__global__ __launch_bounds__(256) void paged_evict_move_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, uint32_t budget, const uint32_t* __restrict__ kept,
-                                                               const uint32_t* __restrict__ cut) {
+__global__ __launch_bounds__(EV_THREADS, 8) void paged_evict_move_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, uint32_t budget, const uint32_t* __restrict__ kept,
+                                                                      const uint32_t* __restrict__ cut) {
     const uint32_t s = blockIdx.z, g = blockIdx.y >> 1, j = threadIdx.x & 7, r0 = threadIdx.x >> 3;
     if (cut[s] == 0) return;
-    KV* const pool = blockIdx.y & 1 ? vp : kp;
-    const uint32_t col = (blockIdx.x * 128 + j * 16) / sizeof(KV);
+    uint8_t* const pool = reinterpret_cast<uint8_t*>(blockIdx.y & 1 ? vp : kp) + blockIdx.x * 128 + j * 16;
     const uint32_t* const idx = kept + (static_cast<uint64_t>(s) * c.n_kv + g) * budget;
-    constexpr uint32_t STEP = EV_ROWS * EV_UNROLL;
-    uint4 row[EV_UNROLL];
     bool ok = true;   // the pages were looked over when the positions were chosen
-    for (uint32_t i0 = 0; i0 < budget; i0 += STEP) {
+    auto at = [&](uint32_t t) { return pool + paged_row<HD>(c, paged_page(c, s, t, ok), g, t) * sizeof(KV); };
+    struct Step {
+        uint4 row[EV_UNROLL];
+        uint32_t from[EV_UNROLL];
+    };
+    auto positions = [&](Step& x, uint32_t i0) __attribute__((always_inline)) {
+#pragma unroll
         for (uint32_t u = 0; u < EV_UNROLL; ++u) {
             const uint32_t i = i0 + u * EV_ROWS + r0;
-            if (i < budget) {
-                const uint32_t t = idx[i];
-                row[u] = *reinterpret_cast<const uint4*>(pool + paged_row<HD>(c, paged_page(c, s, t, ok), g, t) + col);
-            }
+            x.from[u] = i < budget ? idx[i] : i;   // a row that stays where it is needs nothing
         }
-        __syncthreads();   // every row of the step is read
+    };
+    auto read = [&](Step& x, uint32_t i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (uint32_t u = 0; u < EV_UNROLL; ++u)
+            if (x.from[u] != i0 + u * EV_ROWS + r0) x.row[u] = *reinterpret_cast<const uint4*>(at(x.from[u]));
+    };
+    auto write = [&](Step& x, uint32_t i0) __attribute__((always_inline)) {
+        // every wavefront has this step's rows in its registers
+#pragma unroll
+        for (uint32_t u = 0; u < EV_UNROLL; ++u) asm volatile("" : "+v"(x.row[u].x), "+v"(x.row[u].y), "+v"(x.row[u].z), "+v"(x.row[u].w));
+        asm volatile("s_barrier" ::: "memory");
+#pragma unroll
         for (uint32_t u = 0; u < EV_UNROLL; ++u) {
             const uint32_t i = i0 + u * EV_ROWS + r0;
-            if (i < budget) *reinterpret_cast<uint4*>(pool + paged_row<HD>(c, paged_page(c, s, i, ok), g, i) + col) = row[u];
+            if (x.from[u] != i) *reinterpret_cast<uint4*>(at(i)) = x.row[u];
         }
+    };
+    Step a, b;
+#pragma unroll
+    for (uint32_t u = 0; u < EV_UNROLL; ++u) a.row[u] = b.row[u] = make_uint4(0, 0, 0, 0);
+    positions(a, 0);
+    read(a, 0);
+    positions(b, EV_STEP);
+    for (uint32_t i0 = 0; i0 < budget; i0 += 2 * EV_STEP) {
+        read(b, i0 + EV_STEP);
+        write(a, i0);
+        positions(a, i0 + 2 * EV_STEP);
+        read(a, i0 + 2 * EV_STEP);
+        write(b, i0 + EV_STEP);
+        positions(b, i0 + 3 * EV_STEP);
     }
 }
 
@@ -139,7 +176,7 @@ static void paged_evict_launch(cera_hip_ctx* ctx, const cera_hip_paged_kv& c, co
     const PagedView v = paged_view(c, e.max_len);
     hipLaunchKernelGGL(paged_evict_select_kernel, dim3(c.n_kv_heads, c.n_seqs), dim3(EV_THREADS), 0, ctx->stream, v, e.mass, e.mass_stride, e.budget, e.n_first, e.n_recent, kept, e.kept,
                        e.new_lens, cut);
-    hipLaunchKernelGGL((paged_evict_move_kernel<KV, HD>), dim3(HD * sizeof(KV) / 128, 2 * c.n_kv_heads, c.n_seqs), dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v),
+    hipLaunchKernelGGL((paged_evict_move_kernel<KV, HD>), dim3(HD * sizeof(KV) / 128, 2 * c.n_kv_heads, c.n_seqs), dim3(EV_THREADS), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v),
                        e.budget, kept, cut);
 }
 
