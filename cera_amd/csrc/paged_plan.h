@@ -81,7 +81,7 @@ inline PagedCheck verify_check(const cera_hip_verify_draft* d) {
     if (d->vocab == 0 || d->vocab > (1u << 24)) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: a vocabulary of 1 to 2^24 tokens");
     if (d->max_draft == 0 || d->max_draft > 64) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: 1 to 64 drafted tokens");
     if (d->n_seqs > 65535) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: at most 65535 sequences");
-    if (!(d->temperature >= 0) || !std::isfinite(d->temperature)) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: temperature is finite, 0 or more");
+    if (!(d->temperature >= 0 && d->temperature <= 1e6f)) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: a temperature of 0 to 10^6");
     if (d->row_stride && (d->row_stride < d->vocab || d->row_stride > (1ull << 40))) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: row_stride is below the vocabulary");
     for (const void* p : {static_cast<const void*>(d->target), static_cast<const void*>(d->draft), static_cast<const void*>(d->tokens), static_cast<const void*>(d->n_draft),
                           static_cast<const void*>(d->uniform), static_cast<const void*>(d->accepted), static_cast<const void*>(d->out_tokens)})

@@ -567,7 +567,7 @@ CERA_HIP_API cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx*, const cera_
  * A drafted token outside the vocabulary is rejected, and takes nothing away from p. */
 typedef struct {
     uint32_t n_seqs, max_draft, vocab;
-    float temperature;        /* 0 or more */
+    float temperature;        /* 0 to 10^6 */
     uint64_t row_stride;      /* floats between rows of target and draft; 0: vocab */
     const float* target;      /* [n_seqs][max_draft + 1] rows */
     const float* draft;       /* nullable, [n_seqs][max_draft] rows */

@@ -90,6 +90,7 @@ int main() {
     vd(CERA_HIP_ERR_ARGUMENT, "null target", [](auto& x) { x.target = nullptr; });
     vd(CERA_HIP_ERR_ARGUMENT, "temperature", [](auto& x) { x.temperature = -1.0f; });
     vd(CERA_HIP_ERR_ARGUMENT, "temperature NaN", [](auto& x) { x.temperature = NAN; });
+    vd(CERA_HIP_ERR_ARGUMENT, "temperature too high", [](auto& x) { x.temperature = 2e6f; });
     vd(CERA_HIP_ERR_SHAPE, "vocabulary", [](auto& x) { x.vocab = 0; });
     vd(CERA_HIP_ERR_SHAPE, "drafts", [](auto& x) { x.max_draft = 65; });
     vd(CERA_HIP_ERR_SHAPE, "no drafts", [](auto& x) { x.max_draft = 0; });
