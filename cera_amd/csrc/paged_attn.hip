@@ -35,11 +35,11 @@ template <typename KV_, int HD, int CB, bool MASS> struct PagedFew {
     using Shared = PagedShared<NC, HD>;
     template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_attn_part<KV, HD, CB, MASS>(sh, x...); }
 };
-template <int HD> struct PagedMany {
-    using KV = kv_half;
+template <typename KV_, int HD> struct PagedMany {
+    using KV = KV_;
     static constexpr int NC = 128, DIM = HD;
-    using Shared = PagedChunkShared<HD>;
-    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_chunk_part<HD>(sh, x...); }
+    using Shared = PagedChunkShared<KV, HD>;
+    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_chunk_part<KV, HD>(sh, x...); }
 };
 
 // A kv head and group of columns has one list of tiles, sequence after sequence.  Either a workgroup takes a sequence of it, grid =
@@ -249,12 +249,12 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.scale2 = in.scale * 1.44269504088896340736f;
     a.window = in.window; a.n_sink = in.n_sink;
     const uint64_t cols = static_cast<uint64_t>(a.max_queries) * a.G;
-    const bool many = HALF && in.q_first && cols > 48;
+    const bool many = in.q_first && cols > 48;
     const uint32_t cb = HALF && cols > 8 ? 2 : 1;
     a.n_cols = many ? 128 : (HALF ? 8 : 16) * cb;
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
     if (static_cast<uint64_t>(c.n_kv_heads) * a.n_cg > (1u << 23)) return cera_fail(ctx, CERA_HIP_ERR_SHAPE, "paged attention: too many rows of a sequence for one call");
-    a.tile = HALF ? 32 : 16;
+    a.tile = HALF || many ? 32 : 16;
     a.round = std::max(1u, ctx->n_cu / c.n_kv_heads);
     const uint32_t wide = c.n_kv_heads * a.n_cg;
     const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, ctx->n_cu);
@@ -289,9 +289,10 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
         using Work = decltype(tag);
         hipLaunchKernelGGL(paged_attn_kernel<Work>, grid, dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), a, c.n_seqs);
     };
-    if constexpr (HALF) {
-        if (many) launch(PagedMany<HD>{});
-        else if (cb == 2) { if (a.mass) launch(PagedFew<KV, HD, 2, true>{}); else launch(PagedFew<KV, HD, 2, false>{}); }
+    if (many) {
+        launch(PagedMany<KV, HD>{});
+    } else if constexpr (HALF) {
+        if (cb == 2) { if (a.mass) launch(PagedFew<KV, HD, 2, true>{}); else launch(PagedFew<KV, HD, 2, false>{}); }
         else { if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{}); }
     } else {
         if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{});

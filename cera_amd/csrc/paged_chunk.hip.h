@@ -1,23 +1,47 @@
-// Attention of many (row, query head) columns of a kv head over a paged half cache: chunks of new tokens.
+// Attention of many (row, query head) columns of a kv head over a paged cache: chunks of new tokens.
 //
 // The products are those of paged_attn.hip.h in 32 x 32 x 16 form, S^T = K Q^T and O^T = V^T P^T, a wavefront for 32 columns, four of
-// them on the same tiles of 32 positions.  Loads go straight into LDS, the next tile's while this one is multiplied: one barrier a
-// tile.  A row's 16-byte pieces lie at places exchanged by its number, so that neither the keys' reads (a lane per row) nor the
-// values' (transposing reads of 4 rows x 16 dims) meet in a bank; the exchange is made on the way in, by what a lane loads.
+// them on the same tiles of 32 positions in LDS.  A row's 16-byte pieces lie at places exchanged by its number, so that neither the
+// keys' reads (a lane per row) nor the values' (transposing reads of 4 rows x 16 dims) meet in a bank.
 // q and the weights are pairs hi + lo of halves here too, two products each: f32's accuracy at twice the operations.
+// Half cache: loads go straight into LDS, the next tile's while this one is multiplied, one barrier a tile; the exchange is made on the
+// way in, by what a lane loads.
+// F32 cache: keys become pairs of halves on their way into LDS, brought to a largest magnitude below 2^15 by a power of two of each row,
+// which goes into its scores: three products, what is left out is below 2^-21 of one.  Values and weights, whose sum has no room for
+// a power of two a row, become three bfloat16 each, which have f32's range: six products.  All of it takes a quarter of the f32
+// instruction's clocks.
 // What bounds it are the matrix cores, with the softmax between the products in the shadow of the other wavefronts.
 #pragma once
 #include "lds_dma.hip.h"
 #include "paged_attn.hip.h"
 
 typedef float paged_f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 paged_b8 __attribute__((ext_vector_type(8)));
 typedef short paged_s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) paged_s4* paged_lds4;
 
-template <int HD> struct PagedChunkShared {
+template <typename KV, int HD> struct PagedChunkShared;
+template <int HD> struct PagedChunkShared<kv_half, HD> {
     __attribute__((aligned(1024))) uint8_t tile[2][2][32 * HD * 2];   // [buffer][keys, values]
     uint32_t bad;
 };
+template <int HD> struct PagedChunkShared<float, HD> {
+    __attribute__((aligned(1024))) uint8_t tile[1][2][32 * HD * 2];   // keys' and values' first parts
+    __attribute__((aligned(1024))) uint8_t more[3][32 * HD * 2];      // the keys' second part, the values' second and third
+    __attribute__((aligned(16))) int up[32];                          // the power of two of a row of keys
+    uint32_t bad;
+};
+
+// two floats as three bfloat16 each: 24 bits in all
+__device__ __forceinline__ void paged_thirds(float x, float y, uint32_t (&d)[3]) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        const uint32_t a = __builtin_bit_cast(uint32_t, x), b = __builtin_bit_cast(uint32_t, y);
+        d[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        x -= __builtin_bit_cast(float, a & 0xFFFF0000u);
+        y -= __builtin_bit_cast(float, b & 0xFFFF0000u);
+    }
+}
 
 // place of 16-byte piece `piece` in row `row` of a tile
 template <int HD, bool VALUES> __device__ __forceinline__ uint32_t paged_piece(uint32_t row, uint32_t piece) {
@@ -26,10 +50,11 @@ template <int HD, bool VALUES> __device__ __forceinline__ uint32_t paged_piece(u
 }
 
 // Tiles [j_begin, j_end) of sequence s for 128 columns from c0 on; slot: of a part's results.
-template <int HD>
-__device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const PagedView& c, const kv_half* __restrict__ kp, const kv_half* __restrict__ vp, const PagedOp& a, uint32_t g,
+template <typename KV, int HD>
+__device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, const PagedView& c, const KV* __restrict__ kp, const KV* __restrict__ vp, const PagedOp& a, uint32_t g,
                                                  uint32_t cg, uint32_t s, const PagedRows& r, const PagedTiles& tiles, uint32_t c0, uint32_t c_last, uint32_t j_begin, uint32_t j_end,
                                                  uint32_t slot) {
+    constexpr bool PAIRS = sizeof(KV) == 4;              // keys and values too
     constexpr int KS = HD / 16, ND = HD / 32;            // steps over the dims, 32-row tiles of O^T
     constexpr uint32_t ROW = HD * 2, PIECES = HD / 8;    // bytes and 16-byte pieces of a row
     constexpr uint32_t ROWS_KB = 1024 / ROW;             // rows of one load of a wavefront
@@ -41,8 +66,18 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
     const PagedConst<int32_t> table = paged_const(c.table + static_cast<uint64_t>(s) * c.max_pages);
     auto tile_of = [&](uint32_t j) { return (j < tiles.sinks ? j : tiles.main + (j - tiles.sinks)) * 32; };
 
-    // ---- loads: a wavefront has one block of 16 positions of the tile's keys or of its values
+    // ---- loads of a half cache: a wavefront has one block of 16 positions of the tile's keys or of its values
     bool ok = true;
+    auto page_of = [&](uint32_t lo) __attribute__((always_inline)) {   // of a block of 16 positions that some column sees
+        uint32_t page = static_cast<uint32_t>(table[lo >> c.page_log2]);
+        if (page >= c.n_pages) {
+            ok = false;
+            page = 0;
+        }
+        return page * c.page_stride + g * c.head_stride + static_cast<uint64_t>(lo & in_page) * HD;
+    };
+    auto used = [&](uint32_t lo) { return lo <= tiles.P_hi && (lo + 15 >= tiles.start_lo || lo < tiles.sink_hi); };
+    auto live = [&](uint32_t t) { return t <= tiles.P_hi && (t >= tiles.start_lo || t < tiles.sink_hi); };
     const uint32_t blk = w & 1;
     const bool values = w >= 2;
     const uint8_t* const pool = reinterpret_cast<const uint8_t*>(values ? vp : kp);
@@ -55,20 +90,65 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
     const uint32_t dst = lds_addr(sh.tile[0][values]) + blk * 16 * ROW;
     auto load = [&](uint32_t j, uint32_t buf) __attribute__((always_inline)) {
         const uint32_t lo = tile_of(j) + 16 * blk;
-        if (lo <= tiles.P_hi && (lo + 15 >= tiles.start_lo || lo < tiles.sink_hi)) {
-            uint32_t page = static_cast<uint32_t>(table[lo >> c.page_log2]);
-            if (page >= c.n_pages) {
-                ok = false;
-                page = 0;
-            }
-            const uint8_t* const src = lds_dma_base(pool + (page * c.page_stride + g * c.head_stride + static_cast<uint64_t>(lo & in_page) * HD) * 2);
+        if (used(lo)) {
+            const uint8_t* const src = lds_dma_base(pool + page_of(lo) * sizeof(KV));
 #pragma unroll
             for (int k = 0; k < LOADS; ++k) lds_dma_1k(src, off[k], dst + buf * (2 * 32 * ROW) + k * 1024);
         }
     };
+    // ---- of an f32 cache: eight threads a row, its float4 number part, part + 8, ..; wavefronts 0 and 1 have the tile's first block
+    constexpr int NF = HD / 32;
+    const uint32_t f_row = tid >> 3, f_part = tid & 7;
+    float4 fk[PAIRS ? NF : 1], fv[PAIRS ? NF : 1];
+    auto fetch = [&](uint32_t j) __attribute__((always_inline)) {
+        const uint32_t t0 = tile_of(j), lo = t0 + 16 * (w >> 1);
+        const bool in = used(lo);
+        const uint64_t at = (in ? page_of(lo) : 0) + static_cast<uint64_t>(f_row & 15) * HD + 4 * f_part;
+        const bool seen_row = in && live(t0 + f_row);
+#pragma unroll
+        for (int i = 0; i < NF; ++i) {
+            fk[i] = fv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (seen_row) {   // what no column sees may be anything: zeros in its place
+                fk[i] = *reinterpret_cast<const float4*>(kp + at + 32 * i);
+                fv[i] = *reinterpret_cast<const float4*>(vp + at + 32 * i);
+            }
+        }
+    };
+    auto put = [&]() __attribute__((always_inline)) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NF; ++i) top = fmaxf(fmaxf(fmaxf(top, fabsf(fk[i].x)), fmaxf(fabsf(fk[i].y), fabsf(fk[i].z))), fabsf(fk[i].w));
+        top = fmaxf(top, dpp_f<0xB1>(top));
+        top = fmaxf(top, dpp_f<0x4E>(top));
+        top = fmaxf(top, dpp_f<0x141>(top));   // of the row's eight lanes
+        const int up = top > 0.0f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;   // |k| 2^-up < 2^15
+        if constexpr (PAIRS) {
+            if (f_part == 0) sh.up[f_row] = up;
+#pragma unroll
+            for (int i = 0; i < NF; ++i) {
+                const float y[4] = {ldexpf(fk[i].x, -up), ldexpf(fk[i].y, -up), ldexpf(fk[i].z, -up), ldexpf(fk[i].w, -up)};
+                uint32_t hi[2], lo[2], v[2][3];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e], y[2 * e + 1]));
+                    lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16)));
+                }
+                paged_thirds(fv[i].x, fv[i].y, v[0]);
+                paged_thirds(fv[i].z, fv[i].w, v[1]);
+                const uint32_t k_at = f_row * ROW + paged_piece<HD, false>(f_row, (f_part + 8 * i) >> 1) * 16 + (f_part & 1) * 8;
+                const uint32_t v_at = f_row * ROW + paged_piece<HD, true>(f_row, (f_part + 8 * i) >> 1) * 16 + (f_part & 1) * 8;
+                *reinterpret_cast<uint2*>(sh.tile[0][0] + k_at) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(sh.more[0] + k_at) = make_uint2(lo[0], lo[1]);
+                *reinterpret_cast<uint2*>(sh.tile[0][1] + v_at) = make_uint2(v[0][0], v[1][0]);
+                *reinterpret_cast<uint2*>(sh.more[1] + v_at) = make_uint2(v[0][1], v[1][1]);
+                *reinterpret_cast<uint2*>(sh.more[2] + v_at) = make_uint2(v[0][2], v[1][2]);
+            }
+        }
+    };
     if (tid == 0) sh.bad = 0;
     uint32_t j = j_begin, buf = 0;
-    load(j, 0);
+    if constexpr (PAIRS) fetch(j);
+    else load(j, 0);
 
     // ---- the lane's column
     const uint32_t w0 = c0 + 32 * w, col = w0 + lc, cc = min(col, c_last), qi = cc / a.G, h = g * a.G + cc % a.G;
@@ -80,6 +160,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
     const bool idle = w0 > c_last;
     uint4 qh[KS], ql[KS];
     float mul;
+    int q_up;
     {
         const float* const qp = a.q + (r.first + static_cast<uint64_t>(qi)) * a.q_stride + h * HD + 8 * half;
         float top = 0.0f;
@@ -93,7 +174,8 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
         top = fmaxf(top, __shfl_xor(top, 32));
         int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
         up = min(up, 100);
-        mul = ldexpf(fabsf(a.scale2), -up);
+        q_up = up;
+        mul = PAIRS ? fabsf(a.scale2) : ldexpf(fabsf(a.scale2), -up);
         const float sign = a.scale2 < 0.0f ? -1.0f : 1.0f;   // so that the largest product is the largest score
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
@@ -120,21 +202,27 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
     const uint32_t v_row = 4 * half + (lane >> 2 & 3), v_piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), v_byte = 8 * (lane & 1);
 
     for (; j < j_end; ++j, buf ^= 1) {
-        // this tile is in, and every wavefront is past its reads of the other buffer
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
         const uint32_t t0 = tile_of(j);
-        if (t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
-            // values that no column sees may be anything, and 0 times that is not 0
-            for (uint32_t i = tid; i < 32 * PIECES; i += 256) {
-                const uint32_t t = t0 + i / PIECES;
-                if (!(t <= tiles.P_hi && (t >= tiles.start_lo || t < tiles.sink_hi))) *reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16) = make_uint4(0, 0, 0, 0);
-            }
+        if constexpr (PAIRS) {
+            if (j != j_begin) __syncthreads();   // every wavefront is past its reads
+            put();
+            if (j + 1 < j_end) fetch(j + 1);
+            lds_barrier();
+        } else {
+            // this tile is in, and every wavefront is past its reads of the other buffer
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
+            if (t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
+                // values that no column sees may be anything, and 0 times that is not 0
+                for (uint32_t i = tid; i < 32 * PIECES; i += 256)
+                    if (!live(t0 + i / PIECES)) *reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16) = make_uint4(0, 0, 0, 0);
+                __syncthreads();
+            }
+            if (j + 1 < j_end) load(j + 1, buf ^ 1);
         }
-        if (j + 1 < j_end) load(j + 1, buf ^ 1);
         if (idle || t0 > P_hi || (t0 + 31 < seen_lo.start && t0 >= seen_hi.sink_end)) continue;
-        const uint8_t *const kt = sh.tile[buf][0], *const vt = sh.tile[buf][1];
+        const uint32_t now = PAIRS ? 0 : buf;
+        const uint8_t *const kt = sh.tile[now][0], *const vt = sh.tile[now][1];
         paged_f16v x;
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = 0.0f;
@@ -143,6 +231,20 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
             const paged_h8 k = __builtin_bit_cast(paged_h8, *reinterpret_cast<const uint4*>(kt + lc * ROW + paged_piece<HD, false>(lc, 2 * st + half) * 16));
             x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(paged_h8, qh[st]), x, 0, 0, 0);
             x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, __builtin_bit_cast(paged_h8, ql[st]), x, 0, 0, 0);
+            if constexpr (PAIRS) {
+                const paged_h8 kl = __builtin_bit_cast(paged_h8, *reinterpret_cast<const uint4*>(sh.more[0] + lc * ROW + paged_piece<HD, false>(lc, 2 * st + half) * 16));
+                x = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, __builtin_bit_cast(paged_h8, qh[st]), x, 0, 0, 0);
+            }
+        }
+        if constexpr (PAIRS) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int4 up = *reinterpret_cast<const int4*>(&sh.up[8 * i + 4 * half]);
+                x[4 * i] = ldexpf(x[4 * i], up.x - q_up);
+                x[4 * i + 1] = ldexpf(x[4 * i + 1], up.y - q_up);
+                x[4 * i + 2] = ldexpf(x[4 * i + 2], up.z - q_up);
+                x[4 * i + 3] = ldexpf(x[4 * i + 3], up.w - q_up);
+            }
         }
         // product e is of position t0 + 8 (e / 4) + 4 half + e % 4
         const bool edge = !((t0 >= seen_hi.start && t0 + 31 <= P_lo) || t0 + 31 < seen_lo.sink_end);
@@ -176,34 +278,56 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<HD>& sh, const
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) l += x[e];
-        uint4 ph[2], pl[2];
+        // weights as halves (three bfloat16), their products with the values
+        constexpr int NP = PAIRS ? 3 : 2;
+        uint4 p[2][NP];
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
-            uint32_t hi[4], lo[4];
+            uint32_t d[4][NP];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float y0 = x[8 * kk + 2 * e], y1 = x[8 * kk + 2 * e + 1];
-                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
-                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y0) & 0xFFFFE000u),
-                                                                                 y1 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y1) & 0xFFFFE000u)));
+                if constexpr (PAIRS) {
+                    paged_thirds(y0, y1, d[e]);
+                } else {
+                    d[e][0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
+                    d[e][1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y0) & 0xFFFFE000u),
+                                                                                      y1 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y1) & 0xFFFFE000u)));
+                }
             }
-            ph[kk] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            pl[kk] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+#pragma unroll
+            for (int n = 0; n < NP; ++n) p[kk][n] = make_uint4(d[0][n], d[1][n], d[2][n], d[3][n]);
         }
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int i = 0; i < ND; ++i) {
                 // slot e of a half is position 16 kk + 8 (e / 4) + 4 half + e % 4
-                paged_s4 v[2];
+                auto read = [&](const uint8_t* tile) __attribute__((always_inline)) {
+                    paged_s4 v[2];
 #pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    const uint32_t row = 16 * kk + 8 * b + v_row;
-                    v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((paged_lds4)(vt + row * ROW + paged_piece<HD, true>(row, 4 * i + v_piece) * 16 + v_byte));
+                    for (int b = 0; b < 2; ++b) {
+                        const uint32_t row = 16 * kk + 8 * b + v_row;
+                        v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((paged_lds4)(tile + row * ROW + paged_piece<HD, true>(row, 4 * i + v_piece) * 16 + v_byte));
+                    }
+                    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+                if constexpr (PAIRS) {
+                    auto add = [&](paged_b8 v, int n) { o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(paged_b8, p[kk][n]), o[i], 0, 0, 0); };
+                    const paged_b8 v3 = __builtin_bit_cast(paged_b8, read(sh.more[2]));
+                    add(v3, 0);
+                    const paged_b8 v2 = __builtin_bit_cast(paged_b8, read(sh.more[1]));
+                    add(v2, 1);
+                    add(v2, 0);
+                    const paged_b8 v1 = __builtin_bit_cast(paged_b8, read(vt));
+                    add(v1, 2);
+                    add(v1, 1);
+                    add(v1, 0);
+                } else {
+                    const paged_h8 va = __builtin_bit_cast(paged_h8, read(vt));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, p[kk][0]), o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, p[kk][1]), o[i], 0, 0, 0);
                 }
-                const paged_h8 va = __builtin_bit_cast(paged_h8, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, ph[kk]), o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, pl[kk]), o[i], 0, 0, 0);
             }
     }
     l += __shfl_xor(l, 32);

@@ -198,6 +198,31 @@ def test_large_and_small_queries(hip, f16, chunk):
     pool.close()
 
 
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 17, 30]])
+def test_f32_rows_of_very_different_size(hip, counts):
+    """Keys and values that no half can hold, and rows 2^40 apart: the bound is relative to the weighted values' sizes."""
+    lens = [90, 60, 45]
+    r = np.random.default_rng(1)
+    k = [(r.standard_normal((n, 2, 64)) * (2.0 ** r.integers(-20, 3, (n, 2, 1)))).astype(np.float32) for n in lens]
+    v = [(r.standard_normal((n, 2, 64)) * (2.0 ** r.integers(-20, 20, (n, 2, 1)))).astype(np.float32) for n in lens]
+    k[1] *= np.float32(1e6)
+    v[2] *= np.float32(1e20)
+    pool = P.Pool(hip, lens, 2, 64, False, 16, seed=3, k=k, v=v)
+    rows = P.Rows(pool, sum(counts), 8, seed=5)
+    at = counts[0]
+    rows.q[at:at + counts[1]] *= np.float32(1e-6)
+    hip.upload(rows.d_q, rows.q)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    for window in (0, 20):
+        hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first), window=window))
+        got, at = rows.result(), 0
+        for s, m in enumerate(counts):
+            out, bound, _, _ = P.attn_ref(rows.q[at:at + m], k[s], v[s], m, 0.125, window, 0)
+            assert (np.abs(got[at:at + m] - out) <= bound).all(), (s, window)
+            at += m
+    pool.close()
+
+
 def test_offsets_beyond_32_bits(hip):
     """Pages 2^31 elements apart: byte and element offsets past 32 bits."""
     stride, n_kv, hd, page = (1 << 31) + 8, 2, 128, 16
