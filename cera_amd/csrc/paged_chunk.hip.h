@@ -18,6 +18,7 @@
 typedef float paged_f16v __attribute__((ext_vector_type(16)));
 typedef __bf16 paged_b8 __attribute__((ext_vector_type(8)));
 typedef short paged_s4 __attribute__((ext_vector_type(4)));
+typedef short paged_s8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) paged_s4* paged_lds4;
 
 template <typename KV, int HD> struct PagedChunkShared;
@@ -163,29 +164,26 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
     int q_up;
     {
         const float* const qp = a.q + (r.first + static_cast<uint64_t>(qi)) * a.q_stride + h * HD + 8 * half;
+        float4 f[2 * KS];
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) f[i] = *reinterpret_cast<const float4*>(qp + 16 * (i >> 1) + 4 * (i & 1));
         float top = 0.0f;
 #pragma unroll
-        for (int st = 0; st < KS; ++st)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float4 u = *reinterpret_cast<const float4*>(qp + 16 * st + 4 * e);
-                top = fmaxf(fmaxf(fmaxf(top, fabsf(u.x)), fmaxf(fabsf(u.y), fabsf(u.z))), fabsf(u.w));
-            }
+        for (int i = 0; i < 2 * KS; ++i) top = fmaxf(fmaxf(fmaxf(top, fabsf(f[i].x)), fmaxf(fabsf(f[i].y), fabsf(f[i].z))), fabsf(f[i].w));
         top = fmaxf(top, __shfl_xor(top, 32));
         int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
         up = min(up, 100);
         q_up = up;
         mul = PAIRS ? fabsf(a.scale2) : ldexpf(fabsf(a.scale2), -up);
-        const float sign = a.scale2 < 0.0f ? -1.0f : 1.0f;   // so that the largest product is the largest score
+        const float by = ldexpf(a.scale2 < 0.0f ? -1.0f : 1.0f, up);   // the sign too, so that the largest product is the largest score
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
+            const float y[8] = {f[2 * st].x * by, f[2 * st].y * by, f[2 * st].z * by, f[2 * st].w * by, f[2 * st + 1].x * by, f[2 * st + 1].y * by, f[2 * st + 1].z * by, f[2 * st + 1].w * by};
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float2 u = *reinterpret_cast<const float2*>(qp + 16 * st + 2 * e);
-                const float y0 = ldexpf(u.x * sign, up), y1 = ldexpf(u.y * sign, up);
-                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0, y1));
-                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y0 - h2f(hi[e] & 0xFFFF), y1 - h2f(hi[e] >> 16)));
+                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e], y[2 * e + 1]));
+                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16)));
             }
             qh[st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             ql[st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
@@ -246,6 +244,23 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
                 x[4 * i + 3] = ldexpf(x[4 * i + 3], up.w - q_up);
             }
         }
+        // the values of the first 16 positions are on their way while the weights are made
+        auto read = [&](const uint8_t* tile, int kk, int i) __attribute__((always_inline)) {
+            // slot e of a half is position 16 kk + 8 (e / 4) + 4 half + e % 4
+            paged_s4 v[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const uint32_t row = 16 * kk + 8 * b + v_row;
+                v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((paged_lds4)(tile + row * ROW + paged_piece<HD, true>(row, 4 * i + v_piece) * 16 + v_byte));
+            }
+            return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        paged_s8 va[PAIRS ? 1 : ND];
+        if constexpr (!PAIRS) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i) va[i] = read(vt, 0, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         // product e is of position t0 + 8 (e / 4) + 4 half + e % 4
         const bool edge = !((t0 >= seen_hi.start && t0 + 31 <= P_lo) || t0 + 31 < seen_lo.sink_end);
         uint32_t out_of_sight = 0;
@@ -302,31 +317,21 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
         for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
             for (int i = 0; i < ND; ++i) {
-                // slot e of a half is position 16 kk + 8 (e / 4) + 4 half + e % 4
-                auto read = [&](const uint8_t* tile) __attribute__((always_inline)) {
-                    paged_s4 v[2];
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const uint32_t row = 16 * kk + 8 * b + v_row;
-                        v[b] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((paged_lds4)(tile + row * ROW + paged_piece<HD, true>(row, 4 * i + v_piece) * 16 + v_byte));
-                    }
-                    return __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                };
                 if constexpr (PAIRS) {
                     auto add = [&](paged_b8 v, int n) { o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, __builtin_bit_cast(paged_b8, p[kk][n]), o[i], 0, 0, 0); };
-                    const paged_b8 v3 = __builtin_bit_cast(paged_b8, read(sh.more[2]));
+                    const paged_b8 v3 = __builtin_bit_cast(paged_b8, read(sh.more[2], kk, i));
                     add(v3, 0);
-                    const paged_b8 v2 = __builtin_bit_cast(paged_b8, read(sh.more[1]));
+                    const paged_b8 v2 = __builtin_bit_cast(paged_b8, read(sh.more[1], kk, i));
                     add(v2, 1);
                     add(v2, 0);
-                    const paged_b8 v1 = __builtin_bit_cast(paged_b8, read(vt));
+                    const paged_b8 v1 = __builtin_bit_cast(paged_b8, read(vt, kk, i));
                     add(v1, 2);
                     add(v1, 1);
                     add(v1, 0);
                 } else {
-                    const paged_h8 va = __builtin_bit_cast(paged_h8, read(vt));
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, p[kk][0]), o[i], 0, 0, 0);
-                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, __builtin_bit_cast(paged_h8, p[kk][1]), o[i], 0, 0, 0);
+                    const paged_h8 v = __builtin_bit_cast(paged_h8, kk == 0 ? va[i] : read(vt, kk, i));
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(paged_h8, p[kk][0]), o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(paged_h8, p[kk][1]), o[i], 0, 0, 0);
                 }
             }
     }

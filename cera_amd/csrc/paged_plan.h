@@ -125,18 +125,20 @@ PAGED_HD PagedSeen paged_seen(uint32_t P, uint32_t window, uint32_t n_sink) {
     return v;
 }
 
-// How the tiles of a kv head and group of columns are cut among workgroups.  wide: kv heads times groups.
+// How the tiles of a kv head and group of columns are cut among workgroups.  wide: kv heads times groups; chunk: the groups are those of
+// a chunk's many columns.
 struct PagedCut {
     uint32_t spans;   // workgroups, of equal numbers of tiles; 0: one for each sequence
     uint32_t least;   // tiles of a workgroup at least
 };
-inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, uint32_t n_cu) {
+inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, bool chunk, uint32_t n_cu) {
     // tiles that a sequence of max_len may have: those of the window and of the first positions each touch one more at their ends
     uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
     if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
     PagedCut c;
+    // Two workgroups a CU.  Groups of columns that fill the chip by themselves are not cut, nor are short sequences: parts cost a launch
+    // more, and 64 KB each of a chunk's 128 columns written and read again.
     c.least = 256 / tile;
-    // two workgroups a CU; short sequences, and groups of columns that fill the chip by themselves, are not cut
-    c.spans = most <= 384 / tile || n_cu < wide ? 0 : 2 * n_cu / wide;
+    c.spans = most <= (chunk ? 1024 : 384) / tile || n_cu < wide ? 0 : 2 * n_cu / wide;
     return c;
 }
