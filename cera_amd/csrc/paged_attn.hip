@@ -29,11 +29,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __re
 }
 
 // ---- attention ------------------------------------------------------------------------------------------------------
-template <typename KV_, int HD, int CB, bool MASS> struct PagedFew {
+template <typename KV_, int HD, int CB, bool TWIN, bool MASS> struct PagedFew {
     using KV = KV_;
-    static constexpr int NC = (sizeof(KV) == 2 ? 8 : 16) * CB, DIM = HD;
+    static constexpr int NC = (TWIN ? 8 : 16) * CB, DIM = HD;
     using Shared = PagedShared<NC, HD>;
-    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_attn_part<KV, HD, CB, MASS>(sh, x...); }
+    template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_attn_part<KV, HD, CB, TWIN, MASS>(sh, x...); }
 };
 template <typename KV_, int HD> struct PagedMany {
     using KV = KV_;
@@ -249,9 +249,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.scale2 = in.scale * 1.44269504088896340736f;
     a.window = in.window; a.n_sink = in.n_sink;
     const uint64_t cols = static_cast<uint64_t>(a.max_queries) * a.G;
-    const bool many = in.q_first && cols > 48;
-    const uint32_t cb = HALF && cols > 8 ? 2 : 1;
-    a.n_cols = many ? 128 : (HALF ? 8 : 16) * cb;
+    const bool many = in.q_first && cols > (HALF ? 32 : 48);
+    const bool twin = HALF && cols <= 8, two = HALF && cols > 16;
+    a.n_cols = many ? 128 : twin ? 8 : two ? 32 : 16;
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
     if (static_cast<uint64_t>(c.n_kv_heads) * a.n_cg > (1u << 23)) return cera_fail(ctx, CERA_HIP_ERR_SHAPE, "paged attention: too many rows of a sequence for one call");
     a.tile = HALF || many ? 32 : 16;
@@ -292,10 +292,11 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     if (many) {
         launch(PagedMany<KV, HD>{});
     } else if constexpr (HALF) {
-        if (cb == 2) { if (a.mass) launch(PagedFew<KV, HD, 2, true>{}); else launch(PagedFew<KV, HD, 2, false>{}); }
-        else { if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{}); }
+        if (twin) { if (a.mass) launch(PagedFew<KV, HD, 1, true, true>{}); else launch(PagedFew<KV, HD, 1, true, false>{}); }
+        else if (two) { if (a.mass) launch(PagedFew<KV, HD, 2, false, true>{}); else launch(PagedFew<KV, HD, 2, false, false>{}); }
+        else { if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{}); }
     } else {
-        if (a.mass) launch(PagedFew<KV, HD, 1, true>{}); else launch(PagedFew<KV, HD, 1, false>{});
+        if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{});
     }
     if (a.spans || a.mass) {
         const bool shared = a.spans > 8;   // parts of a column shared out

@@ -5,9 +5,10 @@
 //   S^T = K Q^T    A = 16 positions x 32 (f32: 4) dims: a lane loads 16 bytes of its position's row; B = the columns' q.
 //   O^T = V^T P^T  B = the weights in the registers where the scores are: the lane of column c holds positions 4g + r of each 16;
 //                  A = V^T: a lane loads whole pieces of its positions' rows and transposes them in registers (f32: takes them as they are).
-// Half cache: K and V are exact in half precision, q and the weights are pairs hi + lo of halves that take columns c and c + 8 of the
-// 16: f32's accuracy for the price of eight columns a product.  q is brought to a largest magnitude of 2^8 by a power of two, the
-// weights to 2^14, so that low halves stay normal.  F32 cache: the f32 matrix instruction, 16 columns.
+// Half cache: K and V are exact in half precision, q and the weights are pairs hi + lo of halves, for f32's accuracy: with up to eight
+// columns (TWIN) the pair takes columns c and c + 8 of the 16 in one product, else hi and lo have a product each.  q is brought to a
+// largest magnitude of 2^8 by a power of two, the weights to 2^14, so that low halves stay normal.  F32 cache: the f32 matrix
+// instruction, 16 columns.
 // What bounds it is the stream of K and V.
 #pragma once
 #include "paged.hip.h"
@@ -89,19 +90,32 @@ template <int HD> struct PagedTile<float, HD> {
     float4 v[4][VW];
 };
 
+// Two floats as halves.  TWIN: a lane's share of the pair, the high halves (mask 0) or the low ones (mask PAGED_HIGH); else both.
+#define PAGED_HIGH 0xFFFFE000u   // a float's bits that a half holds, rounded towards 0
+template <bool TWIN> __device__ __forceinline__ void paged_pair(float x, float y, uint32_t mask, uint32_t& hi, uint32_t& lo) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, x), b = __builtin_bit_cast(uint32_t, y);
+    if constexpr (TWIN) {
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - __builtin_bit_cast(float, a & mask), y - __builtin_bit_cast(float, b & mask)));
+    } else {
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x, y));
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x - __builtin_bit_cast(float, a & PAGED_HIGH), y - __builtin_bit_cast(float, b & PAGED_HIGH)));
+    }
+}
+
 template <int NC, int HD> struct PagedShared {
     __attribute__((aligned(16))) float o[4][NC][HD + 4];
     float m[4][NC], l[4][NC];
 };
 
 // Tiles [j_begin, j_end) of sequence s for one group of columns, by a workgroup of four wavefronts; slot: of a part's results.
-template <typename KV, int HD, int CB, bool MASS>
-__device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8 : 16) * CB, HD>& sh, const PagedView& c, KV* __restrict__ kp, KV* __restrict__ vp, const PagedOp& a, uint32_t g,
+template <typename KV, int HD, int CB, bool TWIN, bool MASS>
+__device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB, HD>& sh, const PagedView& c, KV* __restrict__ kp, KV* __restrict__ vp, const PagedOp& a, uint32_t g,
                                                 uint32_t cg, uint32_t s, const PagedRows& r, const PagedTiles& tiles, uint32_t c0, uint32_t c_last, uint32_t j_begin, uint32_t j_end, uint32_t slot) {
     constexpr bool HALF = sizeof(KV) == 2;
     using Tile = PagedTile<KV, HD>;
     constexpr int POS = Tile::POS, SUB = Tile::SUB, KS = Tile::KS, NS = 4 * SUB;   // NS: scores of a lane and column block
-    constexpr int CW = HALF ? 8 : 16, NC = CW * CB;
+    static_assert(!TWIN || (HALF && CB == 1), "eight columns and their low halves");
+    constexpr int CW = TWIN ? 8 : 16, NC = CW * CB;
     constexpr int NO = HD / 16;                                                    // 16-row tiles of O^T
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(tid >> 6)));
     const bool alone = j_begin == 0 && j_end == tiles.n;
@@ -211,14 +225,17 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
     }
 
     // ---- the lane's columns
-    const bool low = HALF && (lc & 8);
+    const bool low = TWIN && (lc & 8);
     uint32_t P[CB], start[CB], sink[CB], col[CB];
     float mul[CB];
-    uint4 qh[HALF ? CB : 1][HALF ? KS : 1];
+    // two blocks of pairs are more than the registers hold beside the rest: those lie in LDS, where the results meet later
+    constexpr bool AWAY = HALF && CB == 2;
+    uint4 qh[HALF && !AWAY ? CB : 1][HALF && !AWAY ? KS : 1], ql[HALF && !TWIN && !AWAY ? CB : 1][HALF && !TWIN && !AWAY ? KS : 1];
+    uint4* const q_away = reinterpret_cast<uint4*>(&sh.o[0][0][0]) + lane;   // [block][step][high, low][lane]
     float4 qf[HALF ? 1 : CB][HALF ? 1 : KS];
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
-        col[b] = c0 + b * CW + (HALF ? lc & 7 : lc);
+        col[b] = c0 + b * CW + (TWIN ? lc & 7 : lc);
         const uint32_t cc = min(col[b], c_last), i = cc / a.G, h = g * a.G + cc % a.G;
         P[b] = r.len - r.n + i;
         const PagedSeen v = paged_seen(P[b], a.window, a.n_sink);
@@ -240,17 +257,21 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
             int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
             up = min(up, 100);
             mul[b] = ldexpf(a.scale2, -up);
-            const uint32_t mask = low ? 0xFFFFE000u : 0u;
+            const uint32_t mask = low ? PAGED_HIGH : 0u;
 #pragma unroll
             for (int st = 0; st < KS; ++st) {
-                uint32_t d[4];
+                uint32_t d[4], n[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float y0 = ldexpf(x[st][2 * e], up), y1 = ldexpf(x[st][2 * e + 1], up);
-                    const float z0 = y0 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y0) & mask), z1 = y1 - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y1) & mask);
-                    d[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(z0, z1));
+                for (int e = 0; e < 4; ++e) paged_pair<TWIN>(ldexpf(x[st][2 * e], up), ldexpf(x[st][2 * e + 1], up), mask, d[e], n[e]);
+                if constexpr (AWAY) {
+                    if (w == static_cast<uint32_t>(b)) {
+                        q_away[(2 * (b * KS + st)) * 64] = make_uint4(d[0], d[1], d[2], d[3]);
+                        q_away[(2 * (b * KS + st) + 1) * 64] = make_uint4(n[0], n[1], n[2], n[3]);
+                    }
+                } else {
+                    qh[b][st] = make_uint4(d[0], d[1], d[2], d[3]);
+                    if constexpr (!TWIN) ql[b][st] = make_uint4(n[0], n[1], n[2], n[3]);
                 }
-                qh[b][st] = make_uint4(d[0], d[1], d[2], d[3]);
             }
         } else {
 #pragma unroll
@@ -258,6 +279,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
         }
     }
 
+    if constexpr (AWAY) lds_barrier();
     float m[CB], l[CB];
     paged_f4 o[CB][NO];
 #pragma unroll
@@ -274,7 +296,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
         const bool newest = a.k_new && t0 + POS > tiles.P_hi, more = j + 4 < j_end;
         if (newest) own_key(t0);
         if (more) find(j + 4);
-        uint4 ph[HALF ? CB : 1];
+        uint4 ph[HALF ? CB : 1], pl[HALF && !TWIN ? CB : 1];
         float pf[HALF ? 1 : CB][4];
         float x[CB][NS];
 #pragma unroll
@@ -284,10 +306,22 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
                 paged_f4 d = {0.f, 0.f, 0.f, 0.f};
                 if constexpr (HALF) {
 #pragma unroll
-                    for (int st = 0; st < KS; ++st)
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(paged_h8, f.k[u][st]), __builtin_bit_cast(paged_h8, qh[b][st]), d, 0, 0, 0);
+                    for (int st = 0; st < KS; ++st) {
+                        uint4 hi, lo;
+                        if constexpr (AWAY) {
+                            hi = q_away[(2 * (b * KS + st)) * 64];
+                            lo = q_away[(2 * (b * KS + st) + 1) * 64];
+                        } else {
+                            hi = qh[b][st];
+                            if constexpr (!TWIN) lo = ql[b][st];
+                        }
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(paged_h8, f.k[u][st]), __builtin_bit_cast(paged_h8, hi), d, 0, 0, 0);
+                        if constexpr (!TWIN) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(paged_h8, f.k[u][st]), __builtin_bit_cast(paged_h8, lo), d, 0, 0, 0);
+                    }
+                    if constexpr (TWIN) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[e] += dpp_f<0x128>(d[e]);   // columns c and c + 8: row_ror 8
+                        for (int e = 0; e < 4; ++e) d[e] += dpp_f<0x128>(d[e]);   // columns c and c + 8: row_ror 8
+                    }
                 } else {
 #pragma unroll
                     for (int st = 0; st < KS; ++st) {
@@ -337,15 +371,12 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
                 l[b] += x[b][p];
             }
             if constexpr (HALF) {
-                const uint32_t mask = low ? 0xFFFFE000u : 0u;
-                uint32_t d[4];
+                const uint32_t mask = low ? PAGED_HIGH : 0u;
+                uint32_t d[4], n[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float z0 = x[b][2 * e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[b][2 * e]) & mask),
-                                z1 = x[b][2 * e + 1] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[b][2 * e + 1]) & mask);
-                    d[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(z0, z1));
-                }
+                for (int e = 0; e < 4; ++e) paged_pair<TWIN>(x[b][2 * e], x[b][2 * e + 1], mask, d[e], n[e]);
                 ph[b] = make_uint4(d[0], d[1], d[2], d[3]);
+                if constexpr (!TWIN) pl[b] = make_uint4(n[0], n[1], n[2], n[3]);
             } else {
 #pragma unroll
                 for (int p = 0; p < 4; ++p) pf[b][p] = x[b][p];
@@ -374,7 +405,10 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
                 for (int e = 0; e < 4; ++e) d[e] = __builtin_amdgcn_perm(f.v[2 * e + 1][i >> 1], f.v[2 * e][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
                 const paged_h8 va = __builtin_bit_cast(paged_h8, make_uint4(d[0], d[1], d[2], d[3]));
 #pragma unroll
-                for (int b = 0; b < CB; ++b) o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, __builtin_bit_cast(paged_h8, ph[b]), o[b][i], 0, 0, 0);
+                for (int b = 0; b < CB; ++b) {
+                    o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, __builtin_bit_cast(paged_h8, ph[b]), o[b][i], 0, 0, 0);
+                    if constexpr (!TWIN) o[b][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, __builtin_bit_cast(paged_h8, pl[b]), o[b][i], 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
@@ -408,7 +442,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
     for (int b = 0; b < CB; ++b) {
         l[b] = paged_xor_sum(l[b]);
         if (!ok) l[b] = __builtin_nanf("");
-        const uint32_t lcol = b * CW + (HALF ? lc & 7 : lc);
+        const uint32_t lcol = b * CW + (TWIN ? lc & 7 : lc);
         if (lg == 0 && !low) {
             sh.m[w][lcol] = m[b];
             sh.l[w][lcol] = l[b];
@@ -417,14 +451,14 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(sizeof(KV) == 2 ? 8
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
-        const uint32_t lcol = b * CW + (HALF ? lc & 7 : lc);
+        const uint32_t lcol = b * CW + (TWIN ? lc & 7 : lc);
         const float M = fmaxf(fmaxf(sh.m[0][lcol], sh.m[1][lcol]), fmaxf(sh.m[2][lcol], sh.m[3][lcol])), f0 = __builtin_amdgcn_exp2f(m[b] - M);
 #pragma unroll
         for (int i = 0; i < NO; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 float x = o[b][i][e];
-                if constexpr (HALF) x += dpp_f<0x128>(x);
+                if constexpr (TWIN) x += dpp_f<0x128>(x);
                 const uint32_t d = HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3);
                 if (!low) sh.o[w][lcol][d] = x * f0;
             }
