@@ -131,14 +131,14 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typenam
 }
 
 // ---- the parts of a sequence joined, and weights added up by position ------------------------------------------------
-// grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 2048 positions of a kv head each.
+// grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 1024 positions of a kv head each.
 // Columns: HD / 4 threads of four values for each of SPLIT shares of a column's parts.  Positions: the scores lie as the attention
 // left them, in the base-2 domain.
-static constexpr uint32_t PAGED_MASS_POS = 2048;
+static constexpr uint32_t PAGED_MASS_POS = 1024;
 // part p of a sequence lies this many slots behind slot 2 (its first workgroup)
 __device__ __forceinline__ uint64_t paged_slot(uint32_t p) { return p == 0 ? 1 : 2 * static_cast<uint64_t>(p); }
 template <int HD, int SPLIT>
-__global__ __launch_bounds__(256) void paged_finish_kernel(PagedView c, PagedOp a, uint32_t merge_blocks, uint32_t mass_blocks) {
+__global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, PagedOp a, uint32_t merge_blocks, uint32_t mass_blocks) {
     constexpr uint32_t COLS = 256 / (HD / 4 * SPLIT);
     __shared__ __attribute__((aligned(16))) float4 s_o[SPLIT > 1 ? 256 : 1];
     __shared__ float s_m[SPLIT > 1 ? 256 : 1], s_l[SPLIT > 1 ? 256 : 1];
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(PagedView c, PagedOp 
     if (blockIdx.x < merge_blocks) {
         const uint32_t blocks = (a.n_cols + COLS - 1) / COLS, gx = blockIdx.x / blocks, g = gx / a.n_cg, cg = gx % a.n_cg;
         const uint32_t x = tid % (HD / 4), share = tid / (HD / 4) % SPLIT, lcol = blockIdx.x % blocks * COLS + tid / (HD / 4 * SPLIT), col = cg * a.n_cols + lcol;
-        if (cg * a.n_cols >= n_cols) return;
+        if (cg * a.n_cols + blockIdx.x % blocks * COLS >= n_cols) return;
         const uint2 cut = a.cut[static_cast<uint64_t>(gx) * gridDim.y + s];
         const uint32_t parts = cut.y - cut.x + 1;
         if (parts == 1) return;
@@ -223,13 +223,25 @@ __global__ __launch_bounds__(256) void paged_finish_kernel(PagedView c, PagedOp 
     __syncthreads();
     float* const m = a.mass + (static_cast<uint64_t>(s) * c.n_kv + g) * a.mass_stride;
     const float* const sc = a.scores + (static_cast<uint64_t>(s) * c.n_kv + g) * a.G * a.score_stride;
-    for (uint32_t i = i0 + tid; i < min(n_seen, i0 + PAGED_MASS_POS); i += 256) {
-        const uint32_t t = i < v.sink_end ? i : v.start + (i - v.sink_end);
-        const float before = a.mass_fresh && t == P ? 0.0f : m[t];
-        float sum = 0.0f;
-        for (uint32_t h = 0; h < a.G; ++h) sum = fmaf(__builtin_amdgcn_exp2f(sc[h * a.score_stride + t] - s_h[h]), s_h[a.G + h], sum);
-        if (sum == sum) m[t] = before + sum;
+    // four positions a thread: their loads are in flight together
+    constexpr uint32_t N = PAGED_MASS_POS / 256;
+    uint32_t t[N];
+    float before[N], sum[N];
+#pragma unroll
+    for (uint32_t u = 0; u < N; ++u) {
+        const uint32_t i = min(i0 + u * 256 + tid, n_seen - 1);
+        t[u] = i < v.sink_end ? i : v.start + (i - v.sink_end);
+        before[u] = m[t[u]];
+        sum[u] = 0.0f;
     }
+#pragma unroll 2
+    for (uint32_t h = 0; h < a.G; ++h) {
+#pragma unroll
+        for (uint32_t u = 0; u < N; ++u) sum[u] = fmaf(__builtin_amdgcn_exp2f(sc[h * a.score_stride + t[u]] - s_h[h]), s_h[a.G + h], sum[u]);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < N; ++u)
+        if (i0 + u * 256 + tid < n_seen && sum[u] == sum[u]) m[t[u]] = (a.mass_fresh && t[u] == P ? 0.0f : before[u]) + sum[u];
 }
 
 template <typename KV, int HD>
