@@ -47,6 +47,12 @@ __device__ __forceinline__ uint64_t paged_row(const PagedView& v, uint32_t page,
     return page * v.page_stride + g * v.head_stride + static_cast<uint64_t>(t & ((1u << v.page_log2) - 1)) * HD;
 }
 
+// whether a half of a pair, a float, is infinite or no number
+__device__ __forceinline__ uint32_t paged_odd_halves(uint32_t x) {   // the pair's odd ones as masks of 16 bits
+    return ((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+}
+__device__ __forceinline__ bool paged_odd(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7F800000u) == 0x7F800000u; }
+
 // The context's device while a call lasts: a caller may have made another one current.
 struct PagedDevice {
     int before = -1;

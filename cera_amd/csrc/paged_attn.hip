@@ -269,7 +269,7 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.tile = HALF || many ? 32 : 16;
     a.round = std::max(1u, ctx->n_cu / c.n_kv_heads);
     const uint32_t wide = c.n_kv_heads * a.n_cg;
-    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, many, ctx->n_cu);
+    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, c.n_seqs, many, ctx->n_cu);
     a.spans = cut.spans;
     a.least = cut.least;
     a.score_stride = a.mass ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;

@@ -24,13 +24,13 @@ typedef __attribute__((address_space(3))) paged_s4* paged_lds4;
 template <typename KV, int HD> struct PagedChunkShared;
 template <int HD> struct PagedChunkShared<kv_half, HD> {
     __attribute__((aligned(1024))) uint8_t tile[2][2][32 * HD * 2];   // [buffer][keys, values]
-    uint32_t bad;
+    uint32_t bad, odd[2];   // a bad page; rows of this and of the next tile that hold infinities or NaN which only some columns see
 };
 template <int HD> struct PagedChunkShared<float, HD> {
     __attribute__((aligned(1024))) uint8_t tile[1][2][32 * HD * 2];   // keys' and values' first parts
     __attribute__((aligned(1024))) uint8_t more[3][32 * HD * 2];      // the keys' second part, the values' second and third
     __attribute__((aligned(16))) int up[32];                          // the power of two of a row of keys
-    uint32_t bad;
+    uint32_t bad, odd[2];   // a bad page; rows of this and of the next tile that hold infinities or NaN which only some columns see
 };
 
 // two floats as three bfloat16 each: 24 bits in all
@@ -115,7 +115,25 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             }
         }
     };
-    auto put = [&]() __attribute__((always_inline)) {
+    // 0 times an infinity or NaN is not 0: where only some of the columns see a row, those leave the product and are added behind it
+    auto edge_of_all = [&](uint32_t t0) {
+        return tiles.P_lo != tiles.P_hi && !((t0 >= tiles.start_hi && t0 + 31 <= tiles.P_lo) || t0 + 31 < tiles.sink_lo);
+    };
+    auto put = [&](bool look, uint32_t* odd) __attribute__((always_inline)) {
+        if (look) {
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < (PAIRS ? NF : 1); ++i) {
+                float* const y = &fv[i].x;
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+                    if (paged_odd(y[n])) {
+                        any = true;
+                        y[n] = 0.0f;
+                    }
+            }
+            if (any) atomicOr(odd, 1u << f_row);
+        }
         float top = 0.0f;
 #pragma unroll
         for (int i = 0; i < NF; ++i) top = fmaxf(fmaxf(fmaxf(top, fabsf(fk[i].x)), fmaxf(fabsf(fk[i].y), fabsf(fk[i].z))), fabsf(fk[i].w));
@@ -146,7 +164,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             }
         }
     };
-    if (tid == 0) sh.bad = 0;
+    if (tid == 0) sh.bad = sh.odd[0] = sh.odd[1] = 0;
     uint32_t j = j_begin, buf = 0;
     if constexpr (PAIRS) fetch(j);
     else load(j, 0);
@@ -201,20 +219,36 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
 
     for (; j < j_end; ++j, buf ^= 1) {
         const uint32_t t0 = tile_of(j);
+        uint32_t odd = 0;
         if constexpr (PAIRS) {
-            if (j != j_begin) __syncthreads();   // every wavefront is past its reads
-            put();
+            lds_barrier();   // every wavefront is past its reads, and sh.odd is cleared
+            if (tid == 0) sh.odd[~j & 1] = 0;
+            put(edge_of_all(t0), &sh.odd[j & 1]);
             if (j + 1 < j_end) fetch(j + 1);
             lds_barrier();
+            odd = sh.odd[j & 1];
         } else {
             // this tile is in, and every wavefront is past its reads of the other buffer
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
+            if (tid == 0) sh.odd[~j & 1] = 0;
+            const bool look = edge_of_all(t0);
+            if (look || t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
                 // values that no column sees may be anything, and 0 times that is not 0
-                for (uint32_t i = tid; i < 32 * PIECES; i += 256)
-                    if (!live(t0 + i / PIECES)) *reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16) = make_uint4(0, 0, 0, 0);
+                for (uint32_t i = tid; i < 32 * PIECES; i += 256) {
+                    uint4* const at = reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16);
+                    if (!live(t0 + i / PIECES)) {
+                        *at = make_uint4(0, 0, 0, 0);
+                    } else if (look) {
+                        const uint4 v = *at, o = make_uint4(paged_odd_halves(v.x), paged_odd_halves(v.y), paged_odd_halves(v.z), paged_odd_halves(v.w));
+                        if (o.x | o.y | o.z | o.w) {
+                            *at = make_uint4(v.x & ~o.x, v.y & ~o.y, v.z & ~o.z, v.w & ~o.w);
+                            atomicOr(&sh.odd[j & 1], 1u << (i / PIECES));
+                        }
+                    }
+                }
                 __syncthreads();
+                odd = sh.odd[j & 1];
             }
             if (j + 1 < j_end) load(j + 1, buf ^ 1);
         }
@@ -334,6 +368,20 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
                     o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(paged_h8, p[kk][1]), o[i], 0, 0, 0);
                 }
             }
+        for (odd = __builtin_amdgcn_readfirstlane(odd); odd; odd &= odd - 1) {
+            const uint32_t t = t0 + static_cast<uint32_t>(__builtin_ctz(odd));
+            bool in = true;
+            const KV* const row = vp + paged_row<HD>(c, paged_page(c, s, t, in), g, t) + 4 * half;
+            if (t < seen.sink_end || (t >= seen.start && t <= P)) {
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float y = static_cast<float>(row[32 * i + 8 * (e >> 2) + (e & 3)]);
+                        if (paged_odd(y)) o[i][e] += y;
+                    }
+            }
+        }
     }
     l += __shfl_xor(l, 32);
     if (!ok) sh.bad = 1;

@@ -52,7 +52,8 @@ inline PagedCheck paged_check_attn(const cera_hip_paged_kv* c, const cera_hip_pa
     if (!a || !a->q || !a->out) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: q or out is null");
     if (!a->k_new != !a->v_new) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: k_new and v_new come together");
     if (a->n_heads == 0 || a->n_heads % c->n_kv_heads || a->n_heads > 65536) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: n_heads must be a multiple of n_kv_heads");
-    if (!std::isfinite(a->scale)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: scale must be finite");
+    if (a->n_heads / c->n_kv_heads > 1024) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: at most 1024 query heads a kv head");
+    if (!(std::fabs(a->scale) <= 1e30f)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: scale must be finite, at most 10^30");
     if (!a->q_first && a->n_rows != c->n_seqs) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: without q_first there is one row a sequence");
     if (a->n_rows > (1u << 30)) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: at most 2^30 rows");
     const uint64_t q_row = static_cast<uint64_t>(a->n_heads) * c->head_dim, kv_row = static_cast<uint64_t>(c->n_kv_heads) * c->head_dim;
@@ -131,7 +132,7 @@ struct PagedCut {
     uint32_t spans;   // workgroups, of equal numbers of tiles; 0: one for each sequence
     uint32_t least;   // tiles of a workgroup at least
 };
-inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, bool chunk, uint32_t n_cu) {
+inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, uint32_t n_seqs, bool chunk, uint32_t n_cu) {
     // tiles that a sequence of max_len may have: those of the window and of the first positions each touch one more at their ends
     uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
     if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
@@ -139,6 +140,6 @@ inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t windo
     // Two workgroups a CU.  Groups of columns that fill the chip by themselves are not cut, nor are short sequences: parts cost a launch
     // more, and 64 KB each of a chunk's 128 columns written and read again.
     c.least = 256 / tile;
-    c.spans = most <= (chunk ? 1024 : 384) / tile || n_cu < wide ? 0 : 2 * n_cu / wide;
+    c.spans = most <= (chunk ? 1024 : 384) / tile || n_cu < wide || most * n_seqs > 0x7FFFFFFFu ? 0 : 2 * n_cu / wide;
     return c;
 }

@@ -57,6 +57,8 @@ int main() {
     attn(CERA_HIP_ERR_SHAPE, "heads", [](auto& x) { x.n_heads = 3; });
     attn(CERA_HIP_ERR_SHAPE, "no heads", [](auto& x) { x.n_heads = 0; });
     attn(CERA_HIP_ERR_ARGUMENT, "scale", [](auto& x) { x.scale = INFINITY; });
+    attn(CERA_HIP_ERR_ARGUMENT, "scale too large", [](auto& x) { x.scale = -2e30f; });
+    attn(CERA_HIP_ERR_SHAPE, "heads of a kv head", [](auto& x) { x.n_heads = 2050; });
     attn(CERA_HIP_ERR_SHAPE, "rows", [](auto& x) { x.n_rows = 3; });
     attn(CERA_HIP_ERR_SHAPE, "q stride", [](auto& x) { x.q_stride = 255; });
     attn(CERA_HIP_ERR_SHAPE, "q stride of odd size", [](auto& x) { x.q_stride = 257; });
@@ -117,5 +119,15 @@ int main() {
                     expect(in == got, "what a row sees");
                 }
             }
+    // parts: a kv head's workgroups fit the chip twice, and the count of all tiles fits 32 bits
+    for (uint32_t len : {1u, 300u, 5000u, 1u << 30})
+        for (uint32_t seqs : {1u, 64u, 65535u})
+            for (uint32_t wide : {1u, 8u, 100u, 300u, 5000u})
+                for (uint32_t window : {0u, 1000u, 0xFFFFFFFFu})
+                    for (bool chunk : {false, true}) {
+                        const PagedCut cut = paged_cut(len, 7, window, 4, 32, wide, seqs, chunk, 256);
+                        expect(cut.least >= 1 && static_cast<uint64_t>(cut.spans) * wide <= 512, "parts of a sequence");
+                        expect(cut.spans == 0 || (window && window < len) || (static_cast<uint64_t>(len) + 31) / 32 * seqs < 0x80000000ull, "tiles fit 32 bits");
+                    }
     return failures != 0;
 }

@@ -39,7 +39,7 @@ LENS = [0, 1, 2, 15, 16, 17, 31, 33, 64, 100, 255, 257, 700]
 
 
 @pytest.mark.parametrize("f16", [True, False])
-@pytest.mark.parametrize("heads,n_kv,hd,page", [(32, 8, 128, 64), (28, 4, 128, 16), (12, 2, 64, 32), (4, 4, 64, 256), (8, 1, 128, 128), (18, 2, 64, 16), (20, 1, 128, 32)])
+@pytest.mark.parametrize("heads,n_kv,hd,page", [(32, 8, 128, 64), (28, 4, 128, 16), (12, 2, 64, 32), (4, 4, 64, 256), (8, 1, 128, 128), (18, 2, 64, 16), (20, 1, 128, 32), (40, 1, 64, 64)])
 @pytest.mark.parametrize("window,sinks", [(0, 0), (40, 4), (16, 0), (1, 33), (300, 70)])
 def test_one_token_of_every_sequence(hip, f16, heads, n_kv, hd, page, window, sinks):
     print("decode", f16, heads, n_kv, hd, page, window, sinks, flush=True)
@@ -68,7 +68,7 @@ def test_a_long_sequence_beside_short_ones(hip, f16):
     pool.close()
 
 
-@pytest.mark.parametrize("heads,n_kv,hd,f16", [(32, 8, 128, True), (14, 2, 64, True), (8, 2, 128, False), (20, 1, 64, True)])
+@pytest.mark.parametrize("heads,n_kv,hd,f16", [(32, 8, 128, True), (14, 2, 64, True), (8, 2, 128, False), (20, 1, 64, True), (40, 1, 128, True), (36, 1, 64, False)])
 @pytest.mark.parametrize("window,sinks,fresh", [(0, 0, 0), (0, 0, 1), (100, 6, 1)])
 def test_weights_add_up_by_position(hip, heads, n_kv, hd, f16, window, sinks, fresh):
     lens = [1, 0, 33, 700, 2600]
@@ -221,6 +221,191 @@ def test_f32_rows_of_very_different_size(hip, counts):
             assert (np.abs(got[at:at + m] - out) <= bound).all(), (s, window)
             at += m
     pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("heads,n_kv,hd", [(2, 2, 64), (8, 1, 64), (6, 2, 128), (4, 1, 128), (40, 1, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 2)])
+def test_infinities_reach_only_the_rows_that_see_them(hip, f16, heads, n_kv, hd, window, sinks):
+    """Infinities and NaN among the values, and in keys that no earlier row may see: chunks of few and of many rows."""
+    lens, counts = [70, 150, 40], [6, 50, 3]
+    pool = P.Pool(hip, lens, n_kv, hd, f16, 16, seed=3)
+    k, v = [x.copy() for x in pool.k], [x.copy() for x in pool.v]
+    pool.close()
+    v[0][66, :, 3] = np.inf
+    v[0][67, :, 5] = np.nan
+    v[1][120, :, 7] = -np.inf
+    v[1][140, 0, :] = np.nan
+    k[1][149] = np.nan               # the last row's own key: only it sees it
+    v[2][38, :, hd - 1] = np.inf
+    v[2][39, :, hd - 1] = -np.inf
+    pool = P.Pool(hip, lens, n_kv, hd, f16, 16, seed=3, k=k, v=v)
+    rows = P.Rows(pool, sum(counts), heads, seed=5)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first), window=window, n_sink=sinks))
+    got, at = rows.result(), 0
+    with np.errstate(invalid="ignore"):
+        for s, m in enumerate(counts):
+            out, bound, _, _ = P.attn_ref(rows.q[at:at + m], k[s], v[s], m, 1 / np.sqrt(hd), window, sinks)
+            g = got[at:at + m]
+            if s == 1:
+                assert np.isnan(g[-1]).all()          # its own key is no number
+                g, out, bound = g[:-1], out[:-1], bound[:-1]
+            fine = np.isfinite(out)
+            assert fine.any() and not fine.all()
+            assert (np.abs(g - out)[fine] <= bound[fine]).all(), s
+            # an infinity times a weight's low part of 0 is NaN: what the row sees makes its value not finite, of either kind
+            assert not np.isfinite(g[~fine]).any(), s
+            at += m
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("chunk", [False, True])
+def test_more_sequences_than_a_wavefront_has_lanes(hip, f16, chunk):
+    """150 ragged sequences in equal shares, with empty ones among them, cut and whole."""
+    r = np.random.default_rng(4)
+    lens = [int(x) for x in r.integers(0, 200, 150)]
+    lens[5], lens[77], lens[149], lens[70], lens[0] = 1500, 900, 640, 0, 0
+    counts = [min(n, int(c)) if chunk else 1 for n, c in zip(lens, r.integers(0, 4, 150))]
+    pool = P.Pool(hip, lens, 1, 64, f16, 16, seed=3)
+    rows = P.Rows(pool, sum(counts), 4, seed=4, new=True)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(**(dict(q_first=pool.dev(first), max_queries=3) if chunk else {})))
+    _new_rows(pool, rows, lens, counts)
+    _check(pool, rows, counts, 0, 0)
+    pool.close()
+
+
+@pytest.mark.parametrize("heads,n_kv,f16", [(130, 2, True), (130, 2, False), (300, 1, True)])
+def test_more_heads_of_a_kv_head_than_a_workgroup_has_columns(hip, heads, n_kv, f16):
+    lens = [700, 0, 33, 1]
+    pool = P.Pool(hip, lens, n_kv, 64, f16, 32, seed=11)
+    cap = pool.cols * pool.page
+    d_mass = pool.dev(np.zeros((len(lens), n_kv, cap), np.float32))
+    rows = P.Rows(pool, len(lens), heads, seed=12, new=True)
+    hip.paged_attn(pool.kv(), rows.op(mass=d_mass, mass_stride=cap))
+    _new_rows(pool, rows, lens, [1] * len(lens))
+    masses = _check(pool, rows, [1] * len(lens), 0, 0)
+    for s, n in enumerate(lens):
+        k, v = pool.rows(s, n)
+        assert np.array_equal(k, pool.k[s]) and np.array_equal(v, pool.v[s])
+        mass, mb = masses[s]
+        got = hip.download(d_mass, (len(lens), n_kv, cap), np.float32)[s, :, :n]
+        assert (np.abs(got - mass) <= mb + (1 + heads // n_kv) * 2.0 ** -24 * (mass + 1)).all()
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("chunk", [False, True])
+@pytest.mark.parametrize("scale", [0.0, -0.25, 1e-9, -3.0])
+def test_scales(hip, f16, chunk, scale):
+    """A scale of 0 gives the mean of what is seen; a negative one turns the order round."""
+    lens, counts = [70, 500, 1], [20, 60, 1] if chunk else [1, 1, 1]
+    pool = P.Pool(hip, lens, 1, 64, f16, 16, seed=6)
+    rows = P.Rows(pool, sum(counts), 4, seed=3)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(scale=scale, window=300, **(dict(q_first=pool.dev(first)) if chunk else {})))
+    got, at = rows.result(), 0
+    for s, m in enumerate(counts):
+        out, bound, _, _ = P.attn_ref(rows.q[at:at + m], pool.k[s], pool.v[s], m, scale, 300, 0)
+        assert (np.abs(got[at:at + m] - out) <= bound).all(), s
+        at += m
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("counts", [[3, 2], [30, 20]])
+def test_a_query_that_is_no_number_is_its_row_s_alone(hip, f16, counts):
+    lens = [90, 60]
+    pool = P.Pool(hip, lens, 1, 64, f16, 16, seed=6)
+    rows = P.Rows(pool, sum(counts), 4, seed=3)
+    rows.q[1, 2, 5] = np.nan
+    rows.q[counts[0], 0, 0] = np.inf
+    hip.upload(rows.d_q, rows.q)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first)))
+    got = rows.result().copy()
+    assert np.isnan(got[1, 2]).all() and np.isnan(got[counts[0], 0]).all()
+    for row, h in ((1, 2), (counts[0], 0)):
+        rows.q[row, h] = 0
+        hip.upload(rows.d_q, rows.q)
+    hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first)))
+    want = rows.result()
+    got[1, 2], got[counts[0], 0] = want[1, 2], want[counts[0], 0]
+    assert np.array_equal(got, want)
+    pool.close()
+
+
+def test_without_room_for_parts(hip):
+    """A limit on workspaces: sequences are not cut then, and weights, which need theirs, are refused."""
+    ctx = A.Context(0)
+    lens = [3000, 0, 20]
+    pool = P.Pool(ctx, lens, 2, 64, True, 32, seed=11)
+    cap = pool.cols * pool.page
+    rows = P.Rows(pool, len(lens), 8, seed=12)
+    before = np.ones((len(lens), 2, cap), np.float32)
+    d_mass = pool.dev(before)
+    ctx.set_workspace_limit(4096)
+    ctx.paged_attn(pool.kv(), rows.op())
+    _check(pool, rows, [1] * 3, 0, 0)
+    with pytest.raises(A.HipError) as e:
+        ctx.paged_attn(pool.kv(), rows.op(mass=d_mass, mass_stride=cap))
+    assert e.value.status == 2 and e.value.message
+    assert np.array_equal(ctx.download(d_mass, before.shape, np.float32), before)
+    ctx.set_workspace_limit(0)
+    ctx.paged_attn(pool.kv(), rows.op(mass=d_mass, mass_stride=cap))
+    _check(pool, rows, [1] * 3, 0, 0)
+    got = ctx.download(d_mass, before.shape, np.float32) - 1
+    assert abs(got[0].sum() - 8) < 1e-3 and np.count_nonzero(got[1]) == 0
+    pool.close()
+    ctx.close()
+
+
+def test_two_contexts_and_calls_of_other_sizes_between(hip):
+    """Each context has its own stream and workspaces, and a call's results owe nothing to the calls before it."""
+    import threading
+    ctxs = [A.Context(0), A.Context(0)]
+    work = []
+    for i, ctx in enumerate(ctxs):
+        mine = []
+        for lens in ([2000 + 300 * i, 5, 700], [40, 1, 9 + i], [1200, 1300, 0]):
+            pool = P.Pool(ctx, lens, 2, 128, True, 32, seed=i)
+            rows = P.Rows(pool, 3, 8, seed=i + 5)
+            cap = pool.cols * pool.page
+            mass = pool.dev(np.zeros((3, 2, cap), np.float32))
+            mine.append((pool, rows, mass, cap))
+        work.append(mine)
+    once = [[], []]
+    for i, ctx in enumerate(ctxs):        # each by itself, in order
+        for pool, rows, mass, cap in work[i]:
+            ctx.paged_attn(pool.kv(), rows.op(mass=mass, mass_stride=cap))
+            _check(pool, rows, [1] * 3, 0, 0)
+            once[i].append((rows.result().copy(), ctx.download(mass, (3, 2, cap), np.float32)))
+    wrong = []
+
+    def run(i):
+        try:
+            for k in (2, 1, 0, 1, 2) * 4:
+                pool, rows, mass, cap = work[i][k]
+                ctxs[i].upload(mass, np.zeros((3, 2, cap), np.float32))
+                ctxs[i].paged_attn(pool.kv(), rows.op(mass=mass, mass_stride=cap))
+                out, m = rows.result(), ctxs[i].download(mass, (3, 2, cap), np.float32)
+                if not (np.array_equal(out, once[i][k][0]) and np.array_equal(m, once[i][k][1])):
+                    wrong.append((i, k))
+        except Exception as e:      # a thread's failure is the test's
+            wrong.append(e)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for mine in work:
+        for pool, _, _, _ in mine:
+            pool.close()
+    for ctx in ctxs:
+        ctx.close()
 
 
 def test_offsets_beyond_32_bits(hip):
