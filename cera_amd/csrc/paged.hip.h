@@ -47,11 +47,17 @@ __device__ __forceinline__ uint64_t paged_row(const PagedView& v, uint32_t page,
     return page * v.page_stride + g * v.head_stride + static_cast<uint64_t>(t & ((1u << v.page_log2) - 1)) * HD;
 }
 
-// whether a half of a pair, a float, is infinite or no number
-__device__ __forceinline__ uint32_t paged_odd_halves(uint32_t x) {   // the pair's odd ones as masks of 16 bits
-    return ((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u);
+// Infinities and NaN have the largest exponent: the magnitudes' running maximum, as integers, tells whether any is among many.
+typedef unsigned short paged_u2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t paged_most(uint32_t top, uint32_t pair) {   // of halves, both of a pair at once
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(paged_u2, top), __builtin_bit_cast(paged_u2, pair & 0x7FFF7FFFu)));
 }
+__device__ __forceinline__ uint32_t paged_most(uint32_t top, float x) { return max(top, __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu); }
+__device__ __forceinline__ bool paged_odd_pair(uint32_t x) { return (x & 0x7C00u) == 0x7C00u || (x & 0x7C000000u) == 0x7C000000u; }
 __device__ __forceinline__ bool paged_odd(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7F800000u) == 0x7F800000u; }
+// the value, 0 in the place of such a one
+__device__ __forceinline__ uint32_t paged_even(uint32_t x) { return x & ~(((x & 0x7C00u) == 0x7C00u ? 0xFFFFu : 0u) | ((x & 0x7C000000u) == 0x7C000000u ? 0xFFFF0000u : 0u)); }
+__device__ __forceinline__ float paged_even(float x) { return paged_odd(x) ? 0.0f : x; }
 
 // The context's device while a call lasts: a caller may have made another one current.
 struct PagedDevice {

@@ -1,6 +1,4 @@
 // Attention of new tokens over a paged cache (cera_hip_paged_attn_dev; contract in include/cera_hip.h).
-#include <type_traits>
-
 #include "paged.hip.h"
 #include "paged_attn.hip.h"
 #include "paged_chunk.hip.h"

@@ -396,32 +396,41 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
                     }
                 }
         }
-        // Nor is 0 times an infinity or NaN that only some columns see: those leave the product and are added to theirs behind it.
-        uint32_t odd = 0;   // rows of the tile that have any
+        // Nor is 0 times an infinity or NaN that only some columns see: those leave the product and are added to theirs here.
         if (edge && tiles.P_lo != tiles.P_hi) {
+            uint32_t most = 0;
 #pragma unroll
-            for (int p = 0; p < NS; ++p) {
-                bool any = false;
+            for (int p = 0; p < NS; ++p)
 #pragma unroll
                 for (int e = 0; e < Tile::VW; ++e) {
-                    if constexpr (HALF) {
-                        const uint32_t o16 = paged_odd_halves(f.v[p][e]);
-                        any |= o16 != 0;
-                        f.v[p][e] &= ~o16;
-                    } else {
-                        float* const y = &f.v[p][e].x;
-#pragma unroll
-                        for (int n = 0; n < 4; ++n)
-                            if (paged_odd(y[n])) {
-                                any = true;
-                                y[n] = 0.0f;
-                            }
-                    }
+                    if constexpr (HALF) most = paged_most(most, f.v[p][e]);
+                    else most = paged_most(paged_most(paged_most(paged_most(most, f.v[p][e].x), f.v[p][e].y), f.v[p][e].z), f.v[p][e].w);
                 }
-                const uint64_t lanes = __ballot(any);
+            if (__any(HALF ? paged_odd_pair(most) : paged_odd(__builtin_bit_cast(float, most)))) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-                    if (lanes >> (16 * n) & 0xFFFF) odd |= 1u << (16 * (p >> 2) + 4 * n + (p & 3));
+                for (int p = 0; p < NS; ++p)
+#pragma unroll
+                    for (int e = 0; e < Tile::VW; ++e) {
+                        if constexpr (HALF) f.v[p][e] = paged_even(f.v[p][e]);
+                        else f.v[p][e] = make_float4(paged_even(f.v[p][e].x), paged_even(f.v[p][e].y), paged_even(f.v[p][e].z), paged_even(f.v[p][e].w));
+                    }
+                for (uint32_t t = t0; t < t0 + POS; ++t) {
+                    if (!live(t)) continue;
+                    const uint32_t page = static_cast<uint32_t>(table[t >> c.page_log2]);
+                    const KV* const row = vp + paged_row<HD>(c, page < c.n_pages ? page : 0, g, t);
+#pragma unroll
+                    for (int b = 0; b < CB; ++b)
+                        if (!low && (t < sink[b] || (t >= start[b] && t <= P[b]))) {
+#pragma unroll
+                            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float y = static_cast<float>(row[HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3)]);
+                                    if (paged_odd(y)) o[b][i][e] += y;
+                                    if (e == 3) asm volatile("" ::: "memory");   // few registers: this hardly ever runs
+                                }
+                        }
+                }
             }
         }
         // ---- O^T += V^T P^T
@@ -451,22 +460,6 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
                         o[b][4 * h + 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.z, pf[b][p], o[b][4 * h + 2], 0, 0, 0);
                         o[b][4 * h + 3] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, pf[b][p], o[b][4 * h + 3], 0, 0, 0);
                     }
-                }
-        }
-        for (; odd; odd &= odd - 1) {
-            const uint32_t t = t0 + static_cast<uint32_t>(__builtin_ctz(odd));
-            bool in = true;
-            const KV* const row = vp + paged_row<HD>(c, paged_page(c, s, t, in), g, t);
-#pragma unroll
-            for (int b = 0; b < CB; ++b)
-                if (!low && (t < sink[b] || (t >= start[b] && t <= P[b]))) {
-#pragma unroll
-                    for (int i = 0; i < NO; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float y = static_cast<float>(row[HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3)]);
-                            if (paged_odd(y)) o[b][i][e] += y;
-                        }
                 }
         }
         if (more) load_v();

@@ -12,6 +12,8 @@
 // instruction's clocks.
 // What bounds it are the matrix cores, with the softmax between the products in the shadow of the other wavefronts.
 #pragma once
+#include <type_traits>
+
 #include "lds_dma.hip.h"
 #include "paged_attn.hip.h"
 
@@ -24,13 +26,13 @@ typedef __attribute__((address_space(3))) paged_s4* paged_lds4;
 template <typename KV, int HD> struct PagedChunkShared;
 template <int HD> struct PagedChunkShared<kv_half, HD> {
     __attribute__((aligned(1024))) uint8_t tile[2][2][32 * HD * 2];   // [buffer][keys, values]
-    uint32_t bad, odd[2];   // a bad page; rows of this and of the next tile that hold infinities or NaN which only some columns see
+    uint32_t bad, odd[4];   // a bad page; whether a block of this tile, of the next had infinities or NaN among values that only some columns see
 };
 template <int HD> struct PagedChunkShared<float, HD> {
     __attribute__((aligned(1024))) uint8_t tile[1][2][32 * HD * 2];   // keys' and values' first parts
     __attribute__((aligned(1024))) uint8_t more[3][32 * HD * 2];      // the keys' second part, the values' second and third
     __attribute__((aligned(16))) int up[32];                          // the power of two of a row of keys
-    uint32_t bad, odd[2];   // a bad page; rows of this and of the next tile that hold infinities or NaN which only some columns see
+    uint32_t bad, odd[4];   // a bad page; whether a wavefront's rows of the tile had infinities or NaN among values that only some columns see
 };
 
 // two floats as three bfloat16 each: 24 bits in all
@@ -69,7 +71,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
 
     // ---- loads of a half cache: a wavefront has one block of 16 positions of the tile's keys or of its values
     bool ok = true;
-    auto page_of = [&](uint32_t lo) __attribute__((always_inline)) {   // of a block of 16 positions that some column sees
+    auto page_of = [&](uint32_t lo) __attribute__((always_inline)) {   // element of a position whose block of 16 some column sees
         uint32_t page = static_cast<uint32_t>(table[lo >> c.page_log2]);
         if (page >= c.n_pages) {
             ok = false;
@@ -115,24 +117,20 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             }
         }
     };
-    // 0 times an infinity or NaN is not 0: where only some of the columns see a row, those leave the product and are added behind it
-    auto edge_of_all = [&](uint32_t t0) {
-        return tiles.P_lo != tiles.P_hi && !((t0 >= tiles.start_hi && t0 + 31 <= tiles.P_lo) || t0 + 31 < tiles.sink_lo);
-    };
-    auto put = [&](bool look, uint32_t* odd) __attribute__((always_inline)) {
+    // Tiles that some column sees not all of (a few more may count).  0 times an infinity or NaN is not 0: there, such values leave the
+    // product and are added to the columns that see them apart.
+    const uint32_t look_from = tiles.P_lo < 31 ? 0 : tiles.P_lo - 31, look_below = tiles.start_lo + (tiles.P_hi - tiles.P_lo);
+    auto put = [&](bool look) __attribute__((always_inline)) {
         if (look) {
-            bool any = false;
+            uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < (PAIRS ? NF : 1); ++i) {
-                float* const y = &fv[i].x;
+            for (int i = 0; i < NF; ++i) most = paged_most(paged_most(paged_most(paged_most(most, fv[i].x), fv[i].y), fv[i].z), fv[i].w);
+            const bool odd = __any(paged_odd(__builtin_bit_cast(float, most)));
+            if (lane == 0) sh.odd[w] = odd;
+            if (odd) {
 #pragma unroll
-                for (int n = 0; n < 4; ++n)
-                    if (paged_odd(y[n])) {
-                        any = true;
-                        y[n] = 0.0f;
-                    }
+                for (int i = 0; i < NF; ++i) fv[i] = make_float4(paged_even(fv[i].x), paged_even(fv[i].y), paged_even(fv[i].z), paged_even(fv[i].w));
             }
-            if (any) atomicOr(odd, 1u << f_row);
         }
         float top = 0.0f;
 #pragma unroll
@@ -164,7 +162,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             }
         }
     };
-    if (tid == 0) sh.bad = sh.odd[0] = sh.odd[1] = 0;
+    if (tid == 0) sh.bad = 0;
     uint32_t j = j_begin, buf = 0;
     if constexpr (PAIRS) fetch(j);
     else load(j, 0);
@@ -217,39 +215,50 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
     // where a lane reads: keys by row lc, pieces 2 st + half; values by rows 4 half + (lane & 15) / 4, dims 16 (lane / 16 & 1) + 4 (lane & 3)
     const uint32_t v_row = 4 * half + (lane >> 2 & 3), v_piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), v_byte = 8 * (lane & 1);
 
+    auto add_odd = [&](uint32_t t0) __attribute__((always_inline)) {
+        for (uint32_t t = t0; t < t0 + 32; ++t) {
+            if (!live(t)) continue;
+            const KV* const row = vp + page_of(t) + 4 * half;
+            if (t < seen.sink_end || (t >= seen.start && t <= P)) {
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float y = static_cast<float>(row[32 * i + 8 * (e >> 2) + (e & 3)]);
+                        if (paged_odd(y)) o[i][e] += y;
+                        if ((e & 3) == 3) asm volatile("" ::: "memory");   // few registers: this hardly ever runs
+                    }
+            }
+        }
+    };
+
     for (; j < j_end; ++j, buf ^= 1) {
         const uint32_t t0 = tile_of(j);
-        uint32_t odd = 0;
+        const bool look = t0 >= look_from || t0 < look_below;
         if constexpr (PAIRS) {
-            lds_barrier();   // every wavefront is past its reads, and sh.odd is cleared
-            if (tid == 0) sh.odd[~j & 1] = 0;
-            put(edge_of_all(t0), &sh.odd[j & 1]);
+            if (j != j_begin) lds_barrier();   // every wavefront is past its reads
+            put(look);
             if (j + 1 < j_end) fetch(j + 1);
             lds_barrier();
-            odd = sh.odd[j & 1];
         } else {
-            // this tile is in, and every wavefront is past its reads of the other buffer
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            if (tid == 0) sh.odd[~j & 1] = 0;
-            const bool look = edge_of_all(t0);
-            if (look || t0 + 31 > tiles.P_hi || (t0 < tiles.start_lo && t0 + 31 >= tiles.sink_hi)) {
-                // values that no column sees may be anything, and 0 times that is not 0
-                for (uint32_t i = tid; i < 32 * PIECES; i += 256) {
-                    uint4* const at = reinterpret_cast<uint4*>(sh.tile[buf][1] + i * 16);
-                    if (!live(t0 + i / PIECES)) {
-                        *at = make_uint4(0, 0, 0, 0);
-                    } else if (look) {
-                        const uint4 v = *at, o = make_uint4(paged_odd_halves(v.x), paged_odd_halves(v.y), paged_odd_halves(v.z), paged_odd_halves(v.w));
-                        if (o.x | o.y | o.z | o.w) {
-                            *at = make_uint4(v.x & ~o.x, v.y & ~o.y, v.z & ~o.z, v.w & ~o.w);
-                            atomicOr(&sh.odd[j & 1], 1u << (i / PIECES));
-                        }
-                    }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wavefront's part of the tile is in
+            if (values && look) {   // what no column sees becomes 0
+                uint4* const at = reinterpret_cast<uint4*>(sh.tile[buf][1] + blk * 16 * ROW) + lane;
+                uint4 y[LOADS];
+                uint32_t most = 0;
+#pragma unroll
+                for (int k = 0; k < LOADS; ++k) {
+                    y[k] = at[64 * k];
+                    if (!live(t0 + 16 * blk + k * ROWS_KB + lane / PIECES)) at[64 * k] = y[k] = make_uint4(0, 0, 0, 0);
+                    most = paged_most(paged_most(paged_most(paged_most(most, y[k].x), y[k].y), y[k].z), y[k].w);
                 }
-                __syncthreads();
-                odd = sh.odd[j & 1];
+                const bool odd = __any(paged_odd_pair(most));
+                if (odd)
+#pragma unroll
+                    for (int k = 0; k < LOADS; ++k) at[64 * k] = make_uint4(paged_even(y[k].x), paged_even(y[k].y), paged_even(y[k].z), paged_even(y[k].w));
+                if (lane == 0) sh.odd[2 * (j & 1) + blk] = odd;
             }
+            __syncthreads();   // the tile is whole, and every wavefront is past its reads of the other buffer
             if (j + 1 < j_end) load(j + 1, buf ^ 1);
         }
         if (idle || t0 > P_hi || (t0 + 31 < seen_lo.start && t0 >= seen_hi.sink_end)) continue;
@@ -368,19 +377,9 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
                     o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, __builtin_bit_cast(paged_h8, p[kk][1]), o[i], 0, 0, 0);
                 }
             }
-        for (odd = __builtin_amdgcn_readfirstlane(odd); odd; odd &= odd - 1) {
-            const uint32_t t = t0 + static_cast<uint32_t>(__builtin_ctz(odd));
-            bool in = true;
-            const KV* const row = vp + paged_row<HD>(c, paged_page(c, s, t, in), g, t) + 4 * half;
-            if (t < seen.sink_end || (t >= seen.start && t <= P)) {
-#pragma unroll
-                for (int i = 0; i < ND; ++i)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float y = static_cast<float>(row[32 * i + 8 * (e >> 2) + (e & 3)]);
-                        if (paged_odd(y)) o[i][e] += y;
-                    }
-            }
+        if (look) {
+            const uint32_t* const odd = &sh.odd[PAIRS ? 0 : 2 * (j & 1)];
+            if (odd[0] | odd[1] | (PAIRS ? odd[2] | odd[3] : 0)) add_odd(t0);
         }
     }
     l += __shfl_xor(l, 32);
