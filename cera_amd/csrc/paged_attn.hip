@@ -40,6 +40,42 @@ template <typename KV_, int HD> struct PagedMany {
     template <class... A> __device__ static __forceinline__ void part(Shared& sh, A&&... x) { paged_chunk_part<KV, HD>(sh, x...); }
 };
 
+// Groups of columns that are not cut, of all sequences: the longest first, and every second round of the chip the other way round, so
+// that a CU's add up to about the same.  A group's length is its last position's, or the window: item k is found from the number of
+// groups that are at least 32 L long, for which a lane each looks at its sequence.
+struct PagedItem { uint32_t seq, cg; bool none; };
+__device__ __forceinline__ PagedItem paged_item(const PagedView& c, const PagedOp& a, uint32_t n_seqs, uint32_t k) {
+    const uint32_t lane = threadIdx.x & 63, rows = max(1u, a.n_cols / a.G);   // rows of a group
+    uint32_t len = 0, groups = 0;
+    if (lane < n_seqs) {
+        const PagedRows r = paged_rows(a.q_first, c.lens, lane, a.n_rows, a.max_queries, c.max_len);
+        if (r.n) groups = r.bad || r.len == 0 ? 1 : (r.n * a.G + a.n_cols - 1) / a.n_cols;
+        len = r.bad ? 0 : r.len;
+    }
+    auto sum = [](uint32_t x) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave_sum(static_cast<float>(x))))); };   // below 2^24
+    const uint32_t none = (a.window ? min(c.max_len, a.window) : c.max_len) / 32 + 1;   // the lowest level that no group reaches
+    auto at_least = [&](uint32_t level) { return level == 0 ? groups : level >= none || len < 32 * level ? 0 : min(groups, (len - 32 * level) / rows + 1); };
+    const uint32_t all = sum(groups), in_round = k % a.round, round0 = k - in_round;
+    if (k >= all) return {0, 0, true};
+    if (round0 / a.round & 1) k = round0 + min(a.round, all - round0) - 1 - in_round;
+    // the largest level that more than k groups reach
+    uint32_t lo = 0, hi = none;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (sum(at_least(mid)) > k) lo = mid; else hi = mid;
+    }
+    const uint32_t above = at_least(lo + 1), n = at_least(lo) - above;
+    uint32_t inc = n;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(inc, d);
+        if (lane >= static_cast<uint32_t>(d)) inc += o;
+    }
+    k -= sum(above);
+    const int x = __builtin_ctzll(__ballot(inc > k));
+    const uint32_t i = __builtin_amdgcn_readlane(above, x) + k - __builtin_amdgcn_readlane(inc - n, x);   // from the sequence's last group
+    return {static_cast<uint32_t>(x), static_cast<uint32_t>(__builtin_amdgcn_readlane(groups, x)) - 1 - i, false};
+}
+
 // A kv head and group of columns has one list of tiles, sequence after sequence.  Either a workgroup takes a sequence of it, grid =
 // (kv heads * groups, sequences), or each takes a span of equal length, grid = (kv heads * groups, spans): ragged sequences then cost
 // what their sum costs.  Only the first and the last sequence of a span can be cut: slots 2 span and 2 span + 1.
@@ -48,11 +84,19 @@ template <class Work>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typename Work::KV* __restrict__ kp, typename Work::KV* __restrict__ vp, PagedOp a, uint32_t n_seqs) {
     constexpr int NC = Work::NC;
     __shared__ typename Work::Shared sh;
-    // kv heads side by side, so that a head's workgroups share an XCD's L2 where there are eight; the columns with the most positions first
-    // every second round of the chip the other way, so that a CU's add up to about the same
-    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x % c.n_kv, at_cg = blockIdx.x / c.n_kv, in_round = at_cg % a.round, round0 = at_cg - in_round;
-    const uint32_t cg = a.n_cg - 1 - (round0 / a.round & 1 ? round0 + min(a.round, a.n_cg - round0) - 1 - in_round : at_cg), c0 = cg * NC;
+    // kv heads side by side, so that a head's workgroups share an XCD's L2 where there are eight
+    const uint32_t tid = threadIdx.x, lane = tid & 63, g = blockIdx.x % c.n_kv;
+    uint32_t cg = a.n_cg - 1 - blockIdx.x / c.n_kv;   // the columns with the most positions first
     uint32_t s = blockIdx.y, j = 0, left = 0xFFFFFFFFu, span = 0;   // the sequence, the first of its tiles, tiles left of the span
+    if constexpr (NC == 128) {
+        if (a.ordered) {
+            const PagedItem it = paged_item(c, a, n_seqs, (blockIdx.y * gridDim.x + blockIdx.x) / c.n_kv);
+            if (it.none) return;
+            s = it.seq;
+            cg = it.cg;
+        }
+    }
+    const uint32_t c0 = cg * NC;
     uint32_t s_end = s + 1;
     if (a.spans) {
         span = blockIdx.y;
@@ -267,8 +311,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.tile = HALF || many ? 32 : 16;
     a.round = std::max(1u, ctx->n_cu / c.n_kv_heads);
     const uint32_t wide = c.n_kv_heads * a.n_cg;
-    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, c.n_seqs, many, ctx->n_cu);
+    const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, c.n_seqs, many, HALF, ctx->n_cu);
     a.spans = cut.spans;
+    a.ordered = many && !a.spans && c.n_seqs >= 8 && c.n_seqs <= 64 && wide * c.n_seqs > ctx->n_cu;
     a.least = cut.least;
     a.score_stride = a.mass ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;
     // scores | results of parts | maxima and sums of parts | of whole sequences | who has a sequence's parts

@@ -33,6 +33,7 @@ struct PagedOp {
     uint32_t n_cols, n_cg;                   // columns of a workgroup, groups of them a kv head
     uint32_t tile;                           // positions of a tile
     uint32_t round;                          // groups of a kv head that the chip's CUs have one each of
+    bool ordered;                            // workgroups take uncut groups of all sequences, the longest first
     uint32_t spans, least;                   // workgroups of a kv head and group, and their least number of tiles; spans 0: one for each sequence
     float *acc, *ml;                         // [kv head, group][2 spans][column] x [HD], x (maximum, sum)
     uint2* cut;                              // [kv head, group][seq]: first and last workgroup of a sequence that is cut

@@ -132,14 +132,16 @@ struct PagedCut {
     uint32_t spans;   // workgroups, of equal numbers of tiles; 0: one for each sequence
     uint32_t least;   // tiles of a workgroup at least
 };
-inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, uint32_t n_seqs, bool chunk, uint32_t n_cu) {
+inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t window, uint32_t n_sink, uint32_t tile, uint32_t wide, uint32_t n_seqs, bool chunk, bool half, uint32_t n_cu) {
     // tiles that a sequence of max_len may have: those of the window and of the first positions each touch one more at their ends
     uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
     if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
     PagedCut c;
     // Two workgroups a CU.  Groups of columns that fill the chip by themselves are not cut, nor are short sequences: parts cost a launch
     // more, and 64 KB each of a chunk's 128 columns written and read again.
+    // Up to one uncut workgroup of a chunk a CU: cut shorter ones too.
+    const bool few = static_cast<uint64_t>(wide) * n_seqs <= n_cu;
     c.least = 256 / tile;
-    c.spans = most <= (chunk ? 1024 : 384) / tile || n_cu < wide || most * n_seqs > 0x7FFFFFFFu ? 0 : 2 * n_cu / wide;
+    c.spans = most <= (!chunk ? 384 : !few ? 1024 : half ? 512 : 256) / tile || n_cu < wide || most * n_seqs > 0x7FFFFFFFu ? 0 : 2 * n_cu / wide;
     return c;
 }

@@ -1,9 +1,10 @@
 // Verification of drafted tokens (cera_hip_verify_draft_dev; contract in include/cera_hip.h).
 //
-// A row of logits is cut into chunks.  The first launch writes each chunk's maximum and sum of exponentials; the second forms every
+// A row of logits is cut into chunks.  The first launch writes each chunk's maximum and sum of exponentials.  The second forms every
 // sequence's decision from them (each workgroup for itself) and the chunk sums of the weights that the next token is drawn from; the
-// third finds the chunk and in it the token.  Sums are in 64 bits: the draw compares a running sum over the vocabulary with a
-// random number, and an error e in it moves each of some 10^5 borders by e.  Temperature 0 needs the maxima only: two launches.
+// workgroup of a sequence that is done last finds the chunk and in it the token.  Sums are in 64 bits: the draw compares a running sum
+// over the vocabulary with a random number, and an error e in it moves each of some 10^5 borders by e.  Temperature 0 needs the maxima
+// only.
 #include <cmath>
 
 #include "paged.hip.h"
@@ -12,7 +13,6 @@
 static constexpr uint32_t VD_CHUNK = 1024, VD_THREADS = 256, VD_PER = VD_CHUNK / 64;
 static constexpr uint32_t VD_MAX = 64;   // most drafted tokens
 
-struct VdDecision;
 struct VdArgs {
     const float *target, *draft, *uniform;
     const int32_t* tokens;
@@ -26,7 +26,7 @@ struct VdArgs {
     float* top;        // [row][chunk] maxima; NaN where the chunk holds a NaN or +inf
     uint32_t* arg;     // [row][chunk] (t = 0) the maximum's index
     double* mass;      // [seq][chunk] sums of the weights of the next token
-    VdDecision* decided;   // [seq]
+    uint32_t* done;    // [seq] workgroups that have their sums
 };
 
 // e^((z - top) / t) for z <= top, as 2^k 2^f with k + f = z c - top c, c = log2 e / t, |f| <= 1/2, and 2^f by its Taylor series to
@@ -58,22 +58,37 @@ __device__ __forceinline__ const float* vd_row(const VdArgs& a, uint32_t row) {
     return row < nt ? a.target + row * a.row_stride : a.draft + (row - nt) * a.row_stride;
 }
 
+// a lane's token number e of a chunk: four in a row, 64 lanes side by side
+typedef float vd_float4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ uint32_t vd_token(uint32_t chunk, uint32_t lane, uint32_t e) { return chunk * VD_CHUNK + 256 * (e >> 2) + 4 * lane + (e & 3); }
+
 // grid = (rows, chunks / 4)
 __global__ __launch_bounds__(VD_THREADS) void verify_rows_kernel(VdArgs a) {
     const uint32_t row = blockIdx.x, nt = a.n_seqs * (a.max_draft + 1), lane = threadIdx.x & 63, chunk = blockIdx.y * 4 + (threadIdx.x >> 6);
     const uint32_t s = row < nt ? row / (a.max_draft + 1) : (row - nt) / a.max_draft, i = row < nt ? row % (a.max_draft + 1) : (row - nt) % a.max_draft;
     const uint32_t n = a.n_draft ? a.n_draft[s] : a.max_draft;
+    if (row < nt && i == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.done[s] = 0;
     if (n > a.max_draft || i > n || (row >= nt && i == n) || chunk >= a.n_chunks) return;   // a row that is not asked for
     const float* const z = vd_row(a, row);
-    const uint32_t v0 = chunk * VD_CHUNK + lane;
     float x[VD_PER], top = -__builtin_inff();
     bool bad = false;
-    // all loads at once: without branches
+    // all loads at once, four tokens each: a row need not be aligned to them
+    if (chunk * VD_CHUNK + VD_CHUNK <= a.vocab) {
 #pragma unroll
-    for (uint32_t e = 0; e < VD_PER; ++e) x[e] = z[min(v0 + e * 64, a.vocab - 1)];
+        for (uint32_t e = 0; e < VD_PER; e += 4) {
+            const vd_float4 y = *reinterpret_cast<const vd_float4*>(z + vd_token(chunk, lane, e));
+            x[e] = y.x; x[e + 1] = y.y; x[e + 2] = y.z; x[e + 3] = y.w;
+        }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < VD_PER; ++e) {
+            const uint32_t v = vd_token(chunk, lane, e);
+            x[e] = z[min(v, a.vocab - 1)];
+            x[e] = v < a.vocab ? x[e] : -__builtin_inff();
+        }
+    }
 #pragma unroll
     for (uint32_t e = 0; e < VD_PER; ++e) {
-        x[e] = v0 + e * 64 < a.vocab ? x[e] : -__builtin_inff();
         bad |= !(x[e] < __builtin_inff());
         top = fmaxf(top, x[e]);
     }
@@ -85,7 +100,7 @@ __global__ __launch_bounds__(VD_THREADS) void verify_rows_kernel(VdArgs a) {
     if (a.c == 0.0) {
         uint32_t at = 0xFFFFFFFFu;   // the first that has the maximum
 #pragma unroll
-        for (uint32_t e = VD_PER; e-- > 0;) at = x[e] == top ? v0 + e * 64 : at;
+        for (uint32_t e = VD_PER; e-- > 0;) at = x[e] == top ? vd_token(chunk, lane, e) : at;
         at = mine == top && at < a.vocab ? at : 0xFFFFFFFFu;
         for (int d = 32; d; d >>= 1) at = min(at, static_cast<uint32_t>(__shfl_xor(at, d)));
         if (lane == 0) a.arg[o] = at;
@@ -102,25 +117,45 @@ __global__ __launch_bounds__(VD_THREADS) void verify_rows_kernel(VdArgs a) {
 }
 
 struct VdRow { double top, sum; bool ok; };   // of a whole row
-// by one wavefront, every lane has it
-__device__ __forceinline__ VdRow vd_whole(const VdArgs& a, uint32_t row) {
-    const uint32_t lane = threadIdx.x & 63;
-    const float* const top = a.top + static_cast<uint64_t>(row) * a.n_chunks;
+// 256 chunks' maxima and sums, four a lane
+struct VdPart { float t[4]; double u[4]; };
+__device__ __forceinline__ VdPart vd_part(const VdArgs& a, uint32_t row, uint32_t c0) {
+    const uint64_t at = static_cast<uint64_t>(row) * a.n_chunks;
+    VdPart x;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) x.t[e] = a.top[at + min(c0 + 64 * e + (threadIdx.x & 63), a.n_chunks - 1)];
+    if (a.c != 0.0)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) x.u[e] = a.sum[at + min(c0 + 64 * e + (threadIdx.x & 63), a.n_chunks - 1)];
+    return x;
+}
+// by one wavefront, every lane has it; x: the row's first chunks
+__device__ __forceinline__ VdRow vd_whole(const VdArgs& a, uint32_t row, VdPart x) {
     float m = -__builtin_inff();
+    double sum = 0.0;
     bool bad = false;
-    for (uint32_t c = lane; c < a.n_chunks; c += 64) {
-        const float t = top[c];
-        bad |= t != t;
-        m = fmaxf(m, t);
+    for (uint32_t c0 = 0; c0 < a.n_chunks; c0 += 256) {
+        if (c0) x = vd_part(a, row, c0);
+        float top = -__builtin_inff();
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            bad |= x.t[e] != x.t[e];
+            top = fmaxf(top, x.t[e]);
+        }
+        top = fmaxf(m, wave_max(top));
+        if (a.c == 0.0 || !(top > -__builtin_inff())) {
+            m = top;
+            continue;
+        }
+        const double top_c = top * a.c;
+        if (sum > 0.0) sum *= vd_exp(m, a.c, top_c);
+        m = top;
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if (c0 + 64 * e + (threadIdx.x & 63) < a.n_chunks && x.t[e] > -__builtin_inff()) sum += x.u[e] * vd_exp(x.t[e], a.c, top_c);
     }
-    m = wave_max(m);
     VdRow r{m, 0.0, !__any(bad) && m > -__builtin_inff()};
-    if (!r.ok || a.c == 0.0) return r;
-    const double* const sum = a.sum + static_cast<uint64_t>(row) * a.n_chunks;
-    double v = 0.0;
-    for (uint32_t c = lane; c < a.n_chunks; c += 64)
-        if (top[c] > -__builtin_inff()) v += sum[c] * vd_exp(top[c], a.c, r.top * a.c);
-    r.sum = wave_sum_f64(v);
+    if (r.ok && a.c != 0.0) r.sum = wave_sum_f64(sum);
     return r;
 }
 __device__ __forceinline__ double vd_p(const VdArgs& a, const VdRow& r, float z) { return vd_exp(z, a.c, r.top * a.c) / r.sum; }
@@ -155,9 +190,11 @@ __device__ __forceinline__ VdDecision vd_decide(const VdArgs& a, uint32_t s, VdS
         const uint32_t tok = i < d.n ? static_cast<uint32_t>(a.tokens[static_cast<uint64_t>(s) * a.max_draft + i]) : 0;
         const bool asked = i < d.n && tok < a.vocab && a.c != 0.0;
         const float z = asked ? a.target[row * a.row_stride + tok] : 0.0f, y = asked && a.draft ? a.draft[(drow - nt) * a.row_stride + tok] : 0.0f;
-        const VdRow p = vd_whole(a, row);
+        const bool both = a.draft && i < d.n;
+        const VdPart p0 = vd_part(a, row, 0), q0 = vd_part(a, both ? drow : row, 0);
+        const VdRow p = vd_whole(a, row, p0);
         VdRow q{0.0, 1.0, true};
-        if (a.draft && i < d.n) q = vd_whole(a, drow);
+        if (both) q = vd_whole(a, drow, q0);
         uint8_t v = p.ok && q.ok ? 0 : 2;
         if (a.c == 0.0) {
             if (p.ok && tok == vd_best(a, row, p.top)) v = 1;
@@ -205,57 +242,65 @@ template <uint32_t N> __device__ __forceinline__ void vd_weights(const VdArgs& a
     }
 }
 
-// grid = (chunks / 8, sequences)
-__global__ __launch_bounds__(2 * VD_THREADS) void verify_mass_kernel(VdArgs a) {
-    __shared__ VdShared shd;
-    const uint32_t s = blockIdx.y, chunk = blockIdx.x * 8 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const VdDecision d = vd_decide(a, s, shd);
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.decided[s] = d;
-    if (!d.ok || chunk >= a.n_chunks) return;
-    const float* const z = a.target + (static_cast<uint64_t>(s) * (a.max_draft + 1) + d.j) * a.row_stride;
-    const float* const y = a.draft && d.rest ? a.draft + (static_cast<uint64_t>(s) * a.max_draft + d.j) * a.row_stride : nullptr;
-    double x[VD_PER], sum = 0.0;
-    vd_weights(a, d, z, y, chunk * VD_CHUNK + lane, 64, d.rest, x);
-#pragma unroll
-    for (uint32_t e = 0; e < VD_PER; ++e) sum += x[e];
-    sum = wave_sum_f64(sum);
-    if (lane == 0) a.mass[static_cast<uint64_t>(s) * a.n_chunks + chunk] = sum;
-}
-
 // inclusive running sum over a wavefront's lanes
+template <int CTRL, int ROWS> __device__ __forceinline__ double vd_from(double v) {   // another lane's value, 0 where there is none
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xF, true), hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xF, true);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
 __device__ __forceinline__ double vd_scan(double v) {
-    const uint32_t lane = threadIdx.x & 63;
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(v, d);
-        if (lane >= static_cast<uint32_t>(d)) v += o;
-    }
+    v += vd_from<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+    v += vd_from<0x112, 0xF>(v);
+    v += vd_from<0x114, 0xF>(v);
+    v += vd_from<0x118, 0xF>(v);
+    v += vd_from<0x142, 0xA>(v);   // lanes 15 and 47 to the rows behind them
+    v += vd_from<0x143, 0xC>(v);   // lane 31 to the upper half
     return v;
 }
 
-// grid = sequences
-__global__ __launch_bounds__(VD_THREADS) void verify_pick_kernel(VdArgs a) {
-    __shared__ double wave_sum_of[4], sh_left;
+// grid = (chunks / 8, sequences), temperature 0: (1, sequences).  The weights' sums of eight chunks; the sequence's workgroup that is
+// done last draws the token.
+__global__ __launch_bounds__(2 * VD_THREADS) void verify_pick_kernel(VdArgs a) {
     __shared__ VdShared shd;
-    __shared__ uint32_t sh_chunk, sh_rest, first, last;
-    const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const VdDecision d = a.c == 0.0 ? vd_decide(a, s, shd) : a.decided[s];
+    __shared__ double wave_sum_of[8], sh_left;
+    __shared__ uint32_t sh_chunk, sh_rest, first, last, ticket;
+    const uint32_t s = blockIdx.y, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const VdDecision d = vd_decide(a, s, shd);
     const uint32_t row = s * (a.max_draft + 1) + d.j;
+    const float* const z = a.target + row * a.row_stride;
+    const float* const y = a.draft && d.rest ? a.draft + (static_cast<uint64_t>(s) * a.max_draft + d.j) * a.row_stride : nullptr;
+    double* const m = a.mass + static_cast<uint64_t>(s) * a.n_chunks;
     int32_t next = -1;
     if (d.ok && a.c == 0.0) {
         next = static_cast<int32_t>(vd_best(a, row, d.p.top));
     } else if (d.ok) {
+        const uint32_t mine_chunk = blockIdx.x * 8 + w;
+        if (mine_chunk < a.n_chunks) {
+            double x[VD_PER], sum = 0.0;
+            vd_weights(a, d, z, y, mine_chunk * VD_CHUNK + lane, 64, d.rest, x);
+#pragma unroll
+            for (uint32_t e = 0; e < VD_PER; ++e) sum += x[e];
+            sum = wave_sum_f64(sum);
+            if (lane == 0) __hip_atomic_store(&m[mine_chunk], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every wavefront's sums are out before the ticket is drawn
+        __syncthreads();
+        if (tid == 0) ticket = __hip_atomic_fetch_add(&a.done[s], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (ticket != gridDim.x - 1) return;
         if (w == 0) {
-            const double* const m = a.mass + static_cast<uint64_t>(s) * a.n_chunks;
             auto sum = [&](auto x) {
                 double t = 0.0;
                 for (uint32_t c = lane; c < a.n_chunks; c += 64) t += x(c);
                 return wave_sum_f64(t);
             };
-            double total = sum([&](uint32_t c) { return m[c]; });
+            // as the other workgroups wrote them, whatever this XCD's L2 holds
+            auto weight = [&](uint32_t c) { return __hip_atomic_load(&m[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+            double total = sum(weight);
             // where nothing is left of p - q (p = q but for roundings), p itself
             const bool rest = d.rest && total > 0.0;
             auto chunk = [&](uint32_t c) {
-                if (rest || !d.rest) return m[c];
+                if (rest || !d.rest) return weight(c);
                 const uint64_t o = static_cast<uint64_t>(row) * a.n_chunks + c;
                 return a.top[o] > -__builtin_inff() ? a.sum[o] * vd_p(a, d.p, a.top[o]) : 0.0;
             };
@@ -284,12 +329,10 @@ __global__ __launch_bounds__(VD_THREADS) void verify_pick_kernel(VdArgs a) {
             }
         }
         __syncthreads();
-        const float* const z = a.target + row * a.row_stride;
-        const float* const y = a.draft && d.rest ? a.draft + (static_cast<uint64_t>(s) * a.max_draft + d.j) * a.row_stride : nullptr;
         const bool rest = sh_rest != 0;
         const uint32_t v0 = sh_chunk * VD_CHUNK;
-        // a thread has four tokens in a row
-        constexpr uint32_t N = VD_CHUNK / VD_THREADS;
+        // a thread has two tokens in a row
+        constexpr uint32_t N = VD_CHUNK / (2 * VD_THREADS);
         const uint32_t v1 = v0 + tid * N;
         double x[N], sum = 0.0;
         vd_weights(a, d, z, y, v1, 1, rest, x);
@@ -315,9 +358,11 @@ __global__ __launch_bounds__(VD_THREADS) void verify_pick_kernel(VdArgs a) {
         if (found != 0xFFFFFFFFu) atomicMin(&first, found);
         __syncthreads();
         next = static_cast<int32_t>(first != 0xFFFFFFFFu ? first : last - 1);
+    } else if (blockIdx.x) {
+        return;
     }
     if (tid == 0) a.accepted[s] = d.j;
-    for (uint32_t i = tid; i <= a.max_draft; i += VD_THREADS)
+    for (uint32_t i = tid; i <= a.max_draft; i += 2 * VD_THREADS)
         a.out_tokens[static_cast<uint64_t>(s) * (a.max_draft + 1) + i] = i < d.j ? a.tokens[static_cast<uint64_t>(s) * a.max_draft + i] : i == d.j ? next : -1;
 }
 
@@ -339,15 +384,14 @@ extern "C" cera_hip_status cera_hip_verify_draft_dev(cera_hip_ctx* ctx, const ce
     const uint32_t rows = d->n_seqs * (d->max_draft + 1) + (a.draft ? d->n_seqs * d->max_draft : 0);
     const uint64_t parts = static_cast<uint64_t>(rows) * a.n_chunks;
     void* ws;
-    CERA_TRY(cera_scratch(ctx, 15, parts * 16 + static_cast<uint64_t>(d->n_seqs) * (a.n_chunks * 8 + sizeof(VdDecision)), &ws));
+    CERA_TRY(cera_scratch(ctx, 15, parts * 16 + static_cast<uint64_t>(d->n_seqs) * (a.n_chunks * 8 + 4), &ws));
     a.sum = static_cast<double*>(ws);
     a.mass = a.sum + parts;
-    a.decided = reinterpret_cast<VdDecision*>(a.mass + static_cast<uint64_t>(d->n_seqs) * a.n_chunks);
-    a.top = reinterpret_cast<float*>(a.decided + d->n_seqs);
+    a.top = reinterpret_cast<float*>(a.mass + static_cast<uint64_t>(d->n_seqs) * a.n_chunks);
     a.arg = reinterpret_cast<uint32_t*>(a.top + parts);
+    a.done = a.arg + parts;
     hipLaunchKernelGGL(verify_rows_kernel, dim3(rows, (a.n_chunks + 3) / 4), dim3(VD_THREADS), 0, ctx->stream, a);
-    if (a.c != 0.0) hipLaunchKernelGGL(verify_mass_kernel, dim3((a.n_chunks + 7) / 8, d->n_seqs), dim3(2 * VD_THREADS), 0, ctx->stream, a);
-    hipLaunchKernelGGL(verify_pick_kernel, dim3(d->n_seqs), dim3(VD_THREADS), 0, ctx->stream, a);
+    hipLaunchKernelGGL(verify_pick_kernel, dim3(a.c != 0.0 ? (a.n_chunks + 7) / 8 : 1, d->n_seqs), dim3(2 * VD_THREADS), 0, ctx->stream, a);
     HIP_TRY(ctx, hipGetLastError());
     return CERA_HIP_OK;
 }

@@ -124,9 +124,10 @@ int main() {
         for (uint32_t seqs : {1u, 64u, 65535u})
             for (uint32_t wide : {1u, 8u, 100u, 300u, 5000u})
                 for (uint32_t window : {0u, 1000u, 0xFFFFFFFFu})
-                    for (bool chunk : {false, true}) {
-                        const PagedCut cut = paged_cut(len, 7, window, 4, 32, wide, seqs, chunk, 256);
-                        expect(cut.least >= 1 && static_cast<uint64_t>(cut.spans) * wide <= 512, "parts of a sequence");
+                    for (bool chunk : {false, true})
+                      for (bool half : {false, true}) {
+                        const PagedCut cut = paged_cut(len, 7, window, 4, 32, wide, seqs, chunk, half, 256);
+                        expect(cut.least >= 1 && static_cast<uint64_t>(cut.spans) * wide <= 1024, "parts of a sequence");
                         expect(cut.spans == 0 || (window && window < len) || (static_cast<uint64_t>(len) + 31) / 32 * seqs < 0x80000000ull, "tiles fit 32 bits");
                     }
     return failures != 0;
