@@ -24,6 +24,16 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
     const uint32_t len = c.lens[s];
     const uint64_t sg = static_cast<uint64_t>(s) * c.n_kv + g;
     bool ok = len <= c.max_len;
+    float* const mw = mass + sg * mass_stride;
+    // the middle [lo, hi) of a sequence that is cut has more than `need` positions; its first keys stay in registers between the passes
+    const uint32_t lo = n_first, hi = len - n_recent, need = budget - n_first - n_recent;
+    constexpr uint32_t HELD = 8;
+    uint32_t held[HELD];
+#pragma unroll
+    for (uint32_t u = 0; u < HELD; ++u) {
+        const uint32_t t = lo + tid + u * EV_THREADS;
+        held[u] = ok && len > budget && t < hi ? evict_key(mw[t]) : 0;
+    }
     if (ok)
         for (uint32_t p = tid; p << c.page_log2 < len; p += EV_THREADS) (void)paged_page(c, s, p << c.page_log2, ok);
     ok = __syncthreads_and(ok);
@@ -33,17 +43,6 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
             for (uint32_t i = tid; i < budget; i += EV_THREADS) out[i] = ok && i < len ? static_cast<int32_t>(i) : -1;
         if (g == 0 && tid == 0) { new_lens[s] = len; cut[s] = 0; }
         return;
-    }
-    float* const mw = mass + sg * mass_stride;
-    // the middle [lo, hi) has more than `need` positions
-    const uint32_t lo = n_first, hi = len - n_recent, need = budget - n_first - n_recent;
-    // the first keys stay in registers between the passes
-    constexpr uint32_t HELD = 8;
-    uint32_t held[HELD];
-#pragma unroll
-    for (uint32_t u = 0; u < HELD; ++u) {
-        const uint32_t t = lo + tid + u * EV_THREADS;
-        held[u] = t < hi ? evict_key(mw[t]) : 0;
     }
     // radix selection: `prefix` holds the bits found so far, `left` how many of those that share them still stay
     uint32_t prefix = 0, left = need;
@@ -72,7 +71,11 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
             if (lane == 63) wave_tot[w] = inc;
             __syncthreads();
             uint32_t before = inc - sum;
-            for (uint32_t i = 0; i < w; ++i) before += wave_tot[i];
+#pragma unroll
+            for (uint32_t i = 0; i < EV_THREADS / 64; ++i) {   // all loads in flight
+                const uint32_t x = wave_tot[i];
+                before += i < w ? x : 0;
+            }
             if (before < left && before + sum >= left) {
                 const bool second = before + a < left;
                 sh[0] = prefix | (top - 2 * tid - (second ? 1 : 0)) << shift;
@@ -83,34 +86,47 @@ __global__ __launch_bounds__(EV_THREADS) void paged_evict_select_kernel(PagedVie
             left = sh[1];
         }
     }
-    // in order: larger ones and the ends stay, of the equal ones the first `left`
+    // in order: larger ones and the ends stay, of the equal ones the first `left`; HELD rows of a position a thread at a time
     uint32_t base_gt = 0, base_eq = 0;
     uint32_t* const ws = kept_ws + sg * budget;
-    for (uint32_t t0 = 0; t0 < len; t0 += EV_THREADS) {
-        const uint32_t t = t0 + tid;
-        const bool in = t < len, mid = in && t >= lo && t < hi;
-        const float x = in ? mw[t] : 0.0f;
-        const uint32_t k = evict_key(x);
-        const bool gt = in && (!mid || (need && k > prefix)), eq = mid && need && k == prefix;
-        const uint64_t bg = __ballot(gt), be = __ballot(eq), below = (1ull << lane) - 1;
-        if (lane == 0) wave_tot[w] = __popcll(bg) | __popcll(be) << 16;
+    for (uint32_t t0 = 0; t0 < len; t0 += HELD * EV_THREADS) {
+        float x[HELD];
+        uint64_t bg[HELD], be[HELD];
+#pragma unroll
+        for (uint32_t u = 0; u < HELD; ++u) x[u] = mw[min(t0 + u * EV_THREADS + tid, len - 1)];
+#pragma unroll
+        for (uint32_t u = 0; u < HELD; ++u) {
+            const uint32_t t = t0 + u * EV_THREADS + tid, k = evict_key(x[u]);
+            const bool in = t < len, mid = t >= lo && t < hi;
+            bg[u] = __ballot(in && (!mid || (need && k > prefix)));
+            be[u] = __ballot(in && mid && need && k == prefix);
+            if (lane == 0) hist[u * (EV_THREADS / 64) + w] = __popcll(bg[u]) | __popcll(be[u]) << 16;   // both at most 64 * 128 when added up
+        }
         __syncthreads();
-        uint32_t sg_ = 0, se_ = 0, tg = 0, te = 0;
-        for (uint32_t i = 0; i < EV_THREADS / 64; ++i) {
-            const uint32_t v = wave_tot[i];
-            if (i < w) { sg_ += v & 0xFFFF; se_ += v >> 16; }
-            tg += v & 0xFFFF;
-            te += v >> 16;
+        // running sums over the step's 128 wavefronts and rows
+        const uint32_t c0 = hist[2 * lane], c1 = hist[2 * lane + 1];
+        uint32_t inc = c0 + c1;
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(inc, d);
+            if (lane >= static_cast<uint32_t>(d)) inc += o;
         }
-        const uint32_t n_gt = base_gt + sg_ + __popcll(bg & below), n_eq = base_eq + se_ + __popcll(be & below);
-        if (gt || (eq && n_eq < left)) {
-            const uint32_t dst = n_gt + min(n_eq, left);
-            ws[dst] = t;
-            if (out) out[dst] = static_cast<int32_t>(t);
-            mw[dst] = x;   // dst <= t, and all of this step's weights are read
+        const uint32_t first = inc - c0 - c1, below = first + c0;   // in front of entries 2 lane, 2 lane + 1
+#pragma unroll
+        for (uint32_t u = 0; u < HELD; ++u) {
+            const uint32_t at = u * (EV_THREADS / 64) + w, v = w & 1 ? __shfl(below, at >> 1) : __shfl(first, at >> 1);
+            const uint64_t under = (1ull << lane) - 1;
+            const uint32_t n_gt = base_gt + (v & 0xFFFF) + __popcll(bg[u] & under), n_eq = base_eq + (v >> 16) + __popcll(be[u] & under);
+            const bool gt = bg[u] >> lane & 1, eq = be[u] >> lane & 1;
+            if (gt || (eq && n_eq < left)) {
+                const uint32_t t = t0 + u * EV_THREADS + tid, dst = n_gt + min(n_eq, left);
+                ws[dst] = t;
+                if (out) out[dst] = static_cast<int32_t>(t);
+                mw[dst] = x[u];   // dst <= t, and all of this step's weights are read
+            }
         }
-        base_gt += tg;
-        base_eq += te;
+        const uint32_t all = __shfl(inc, 63);
+        base_gt += all & 0xFFFF;
+        base_eq += all >> 16;
         __syncthreads();
     }
     if (g == 0 && tid == 0) { new_lens[s] = budget; cut[s] = len; }
