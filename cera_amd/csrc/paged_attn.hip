@@ -331,7 +331,7 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.ml = a.acc + parts() * HD;
     a.ml_seq = a.ml + parts() * 2;
     a.cut = reinterpret_cast<uint2*>(a.ml_seq + ml_seq);
-    if (in.k_new && in.q_first) {
+    if (in.k_new && many) {
         const uint64_t items = static_cast<uint64_t>(a.max_queries) * c.n_kv_heads * (HD / 4);
         hipLaunchKernelGGL((paged_append_kernel<KV, HD>), dim3(static_cast<uint32_t>(std::min<uint64_t>((items + 255) / 256, 1024)), c.n_seqs), dim3(256), 0, ctx->stream, v,
                            static_cast<KV*>(c.k), static_cast<KV*>(c.v), in.k_new, in.v_new, a.kv_stride, a.q_first, a.n_rows, a.max_queries);

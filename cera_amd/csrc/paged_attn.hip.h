@@ -27,7 +27,7 @@ struct PagedOp {
     uint32_t n_rows, max_queries, G;
     float scale2;   // times log2 e
     uint32_t window, n_sink;
-    const float *k_new, *v_new;              // decode form: the rows' own keys and values, or null
+    const float *k_new, *v_new;              // few columns: the rows' own keys and values, or null
     uint64_t kv_stride;
     uint32_t mass_fresh;
     uint32_t n_cols, n_cg;                   // columns of a workgroup, groups of them a kv head
@@ -176,14 +176,16 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
             }
         }
     };
-    // The decode step's own row is not in its page yet: lanes that hold a piece of it take that from the new rows, narrowed as the
-    // cache's.
-    const uint64_t own = r.first * a.kv_stride + g * HD;
+    // The call's own rows, positions new0 on, are not in their pages yet: lanes that hold a piece of one take it from the new rows,
+    // narrowed as the cache's.
+    const uint32_t new0 = r.len - r.n;
+    auto own_row = [&](const float* rows, uint32_t t) { return rows + (r.first + static_cast<uint64_t>(t - new0)) * a.kv_stride + g * HD; };
     auto own_key = [&](uint32_t t0) __attribute__((always_inline)) {
-        const float* const kn = a.k_new + own + lg * (16 / sizeof(KV));
 #pragma unroll
-        for (int u = 0; u < SUB; ++u)
-            if (t0 + 16 * u + lc == tiles.P_hi) {
+        for (int u = 0; u < SUB; ++u) {
+            const uint32_t t = t0 + 16 * u + lc;
+            if (t >= new0 && t <= tiles.P_hi) {
+                const float* const kn = own_row(a.k_new, t) + lg * (16 / sizeof(KV));
 #pragma unroll
                 for (int st = 0; st < KS; ++st) {
                     if constexpr (HALF) {
@@ -194,24 +196,22 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
                     }
                 }
             }
+        }
     };
     auto own_value = [&](uint32_t t0) __attribute__((always_inline)) {
-        const float* const vn = a.v_new + own + lc * (HALF ? HD / 16 : 4);
-        const uint32_t p0 = tiles.P_hi - t0;   // the row's place in the tile
-        if (lg == (p0 >> 2 & 3)) {
 #pragma unroll
-            for (int e = 0; e < Tile::VW; ++e) {
-                if constexpr (HALF) {
-                    const float2 y = *reinterpret_cast<const float2*>(vn + 2 * e);
-                    const uint32_t d = f2h(y.x) | f2h(y.y) << 16;
+        for (int p = 0; p < NS; ++p) {
+            const uint32_t t = t0 + 16 * (p >> 2) + 4 * lg + (p & 3);
+            if (t >= new0 && t <= tiles.P_hi) {
+                const float* const vn = own_row(a.v_new, t) + lc * (HALF ? HD / 16 : 4);
 #pragma unroll
-                    for (int p = 0; p < NS; ++p)
-                        if (static_cast<uint32_t>(p) == ((p0 >> 4) << 2 | (p0 & 3))) f.v[p][e] = d;
-                } else {
-                    const float4 y = *reinterpret_cast<const float4*>(vn + 64 * e);
-#pragma unroll
-                    for (int p = 0; p < NS; ++p)
-                        if (static_cast<uint32_t>(p) == (p0 & 3)) f.v[p][e] = y;
+                for (int e = 0; e < Tile::VW; ++e) {
+                    if constexpr (HALF) {
+                        const float2 y = *reinterpret_cast<const float2*>(vn + 2 * e);
+                        f.v[p][e] = f2h(y.x) | f2h(y.y) << 16;
+                    } else {
+                        f.v[p][e] = *reinterpret_cast<const float4*>(vn + 64 * e);
+                    }
                 }
             }
         }
@@ -294,7 +294,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
     for (; j < j_end; j += 4) {
         const uint32_t t0 = tile_of(j);
         const bool edge = !whole(t0);
-        const bool newest = a.k_new && t0 + POS > tiles.P_hi, more = j + 4 < j_end;
+        const bool newest = a.k_new && t0 + POS > new0, more = j + 4 < j_end;
         if (newest) own_key(t0);
         if (more) find(j + 4);
         uint4 ph[HALF ? CB : 1], pl[HALF && !TWIN ? CB : 1];
@@ -419,6 +419,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
                     if (!live(t)) continue;
                     const uint32_t page = static_cast<uint32_t>(table[t >> c.page_log2]);
                     const KV* const row = vp + paged_row<HD>(c, page < c.n_pages ? page : 0, g, t);
+                    const float* const vn = a.k_new && t >= new0 ? own_row(a.v_new, t) : nullptr;
 #pragma unroll
                     for (int b = 0; b < CB; ++b)
                         if (!low && (t < sink[b] || (t >= start[b] && t <= P[b]))) {
@@ -426,7 +427,8 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
                             for (int i = 0; i < NO; ++i)
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const float y = static_cast<float>(row[HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3)]);
+                                    const uint32_t dim = HALF ? (4 * lg + e) * (HD / 16) + i : 64 * (i >> 2) + 4 * (4 * lg + e) + (i & 3);
+                                    const float y = vn ? static_cast<float>(static_cast<KV>(vn[dim])) : static_cast<float>(row[dim]);
                                     if (paged_odd(y)) o[b][i][e] += y;
                                     if (e == 3) asm volatile("" ::: "memory");   // few registers: this hardly ever runs
                                 }
@@ -467,14 +469,14 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // ---- the new row into its page, by the wavefront that had its tile
-    if (a.k_new && cg == 0 && j_end == tiles.n && (tiles.n - 1 - j_begin) % 4 == w && lane < HD / 2) {
-        bool in = true;
-        const uint32_t page = paged_page(c, s, tiles.P_hi, in), c4 = lane % (HD / 4);
-        if (in)
-            KvOps<KV>::st4((lane < HD / 4 ? kp : vp) + paged_row<HD>(c, page, g, tiles.P_hi), c4,
-                           *reinterpret_cast<const float4*>((lane < HD / 4 ? a.k_new : a.v_new) + r.first * a.kv_stride + g * HD + 4 * c4));
-    }
+    // ---- the new rows into their pages, by the workgroup that has the last one's tile
+    if (a.k_new && cg == (r.n * a.G - 1) / NC && j_end == tiles.n)
+        for (uint32_t i = tid; i < r.n * (HD / 2); i += 256) {
+            const uint32_t t = new0 + i / (HD / 2), part = i % (HD / 2), c4 = part % (HD / 4);
+            bool in = true;
+            const uint32_t page = paged_page(c, s, t, in);
+            if (in) KvOps<KV>::st4((part < HD / 4 ? kp : vp) + paged_row<HD>(c, page, g, t), c4, *reinterpret_cast<const float4*>(own_row(part < HD / 4 ? a.k_new : a.v_new, t) + 4 * c4));
+        }
     // ---- the four wavefronts joined
 #pragma unroll
     for (int b = 0; b < CB; ++b) {

@@ -261,6 +261,37 @@ def test_infinities_reach_only_the_rows_that_see_them(hip, f16, heads, n_kv, hd,
 
 
 @pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("heads,n_kv,hd", [(2, 2, 64), (8, 1, 64), (4, 1, 128), (40, 1, 128)])
+@pytest.mark.parametrize("window", [0, 2])
+def test_new_values_that_are_not_finite(hip, f16, heads, n_kv, hd, window):
+    """Among a chunk's own rows, one of them infinite only as the cache holds it."""
+    lens, counts = [70, 53, 4], [5, 40, 2]
+    pool = P.Pool(hip, lens, n_kv, hd, f16, 16, seed=3)
+    rows = P.Rows(pool, sum(counts), heads, seed=5, new=True)
+    rows.v_new[2, :, 3] = np.inf
+    rows.v_new[3, :, 5] = 1e6
+    rows.v_new[4, :, 6] = np.nan
+    rows.v_new[5 + 30, 0, :9] = -np.inf
+    rows.v_new[46, :, hd - 1] = -1e6
+    hip.upload(rows.d_vn, rows.v_new)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    with np.errstate(over="ignore", invalid="ignore"):
+        _new_rows(pool, rows, lens, counts)
+        hip.paged_attn(pool.kv(), rows.op(q_first=pool.dev(first), window=window))
+        got, at = rows.result(), 0
+        for s, m in enumerate(counts):
+            out, bound, _, _ = P.attn_ref(rows.q[at:at + m], pool.k[s], pool.v[s], m, 1 / np.sqrt(hd), window, 0)
+            fine = np.isfinite(out)
+            assert fine.any() and (fine.all() if s == 2 and not f16 else not fine.all())
+            assert (np.abs(got[at:at + m] - out)[fine] <= bound[fine]).all() and not np.isfinite(got[at:at + m][~fine]).any(), s
+            at += m
+    for s, n in enumerate(lens):
+        k, v = pool.rows(s, n)
+        assert np.array_equal(k, pool.k[s]) and np.array_equal(v, pool.v[s], equal_nan=True)
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("chunk", [False, True])
 def test_more_sequences_than_a_wavefront_has_lanes(hip, f16, chunk):
     """150 ragged sequences in equal shares, with empty ones among them, cut and whole."""
