@@ -187,28 +187,30 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
     extern __shared__ float s_h[];   // [G] maximum, [G] 1 / sum
     const uint32_t s = blockIdx.y, tid = threadIdx.x;
     const PagedRows r = paged_rows(a.q_first, c.lens, s, a.n_rows, a.max_queries, c.max_len);
+    const bool merge = blockIdx.x < merge_blocks;
+    const uint32_t blocks = (a.n_cols + COLS - 1) / COLS, gx = merge ? blockIdx.x / blocks : 0;
+    const uint2 cut = merge ? a.cut[static_cast<uint64_t>(gx) * gridDim.y + s] : make_uint2(0, 0);   // on its way beside the lengths
     if (r.bad || r.len == 0) return;   // written by the attention's launch
     const uint32_t n_cols = r.n * a.G;
-    if (blockIdx.x < merge_blocks) {
-        const uint32_t blocks = (a.n_cols + COLS - 1) / COLS, gx = blockIdx.x / blocks, g = gx / a.n_cg, cg = gx % a.n_cg;
+    if (merge) {
+        const uint32_t g = gx / a.n_cg, cg = gx % a.n_cg;
         const uint32_t x = tid % (HD / 4), share = tid / (HD / 4) % SPLIT, lcol = blockIdx.x % blocks * COLS + tid / (HD / 4 * SPLIT), col = cg * a.n_cols + lcol;
         if (cg * a.n_cols + blockIdx.x % blocks * COLS >= n_cols) return;
-        const uint2 cut = a.cut[static_cast<uint64_t>(gx) * gridDim.y + s];
         const uint32_t parts = cut.y - cut.x + 1;
         if (parts == 1) return;
         const bool mine = lcol < a.n_cols && col < n_cols;
         const uint64_t first = (static_cast<uint64_t>(gx) * 2 * a.spans + 2 * cut.x) * a.n_cols + (mine ? lcol : 0);
-        float M = PAGED_LOWEST;
-        for (uint32_t p = share; p < parts; p += SPLIT) M = fmaxf(M, a.ml[(first + paged_slot(p) * a.n_cols) * 2]);
-        float L = 0.0f;
+        float M = PAGED_LOWEST, L = 0.0f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (uint32_t p = share; p < parts; p += SPLIT) {
             const uint64_t at = first + paged_slot(p) * a.n_cols;
-            const float f = __builtin_amdgcn_exp2f(a.ml[at * 2] - M);
+            const float2 y_ml = *reinterpret_cast<const float2*>(a.ml + at * 2);
             const float4 y = *reinterpret_cast<const float4*>(a.acc + at * HD + 4 * x);
-            L = fmaf(f, a.ml[at * 2 + 1], L);
-            o.x = fmaf(f, y.x, o.x); o.y = fmaf(f, y.y, o.y); o.z = fmaf(f, y.z, o.z); o.w = fmaf(f, y.w, o.w);
+            const float m = fmaxf(M, y_ml.x), f0 = __builtin_amdgcn_exp2f(M - m), f = __builtin_amdgcn_exp2f(y_ml.x - m);
+            M = m;
+            L = fmaf(f, y_ml.y, L * f0);
+            o.x = fmaf(f, y.x, o.x * f0); o.y = fmaf(f, y.y, o.y * f0); o.z = fmaf(f, y.z, o.z * f0); o.w = fmaf(f, y.w, o.w * f0);
         }
         if constexpr (SPLIT > 1) {
             s_o[tid] = o;
@@ -238,34 +240,9 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
     const PagedSeen v = paged_seen(P, a.window, a.n_sink);
     const uint32_t n_seen = v.sink_end + (P + 1 - v.start);
     if (i0 >= n_seen) return;
-    for (uint32_t h = tid >> 6; h < a.G; h += 4) {   // a wavefront per head, its lanes over the parts
-        const uint32_t cg = h / a.n_cols;
-        const uint64_t gx = g * a.n_cg + cg;
-        const uint2 cut = a.spans ? a.cut[gx * gridDim.y + s] : make_uint2(0, 0);
-        float M = PAGED_LOWEST, L = 0.0f;
-        if (cut.x == cut.y) {
-            const float* const ml = a.ml_seq + ((gx * gridDim.y + s) * a.n_cols + h % a.n_cols) * 2;
-            M = ml[0];
-            L = ml[1];
-        } else {
-            const uint64_t first = (gx * 2 * a.spans + 2 * cut.x) * a.n_cols + h % a.n_cols;
-            for (uint32_t p = tid & 63; p <= cut.y - cut.x; p += 64) M = fmaxf(M, a.ml[(first + paged_slot(p) * a.n_cols) * 2]);
-            M = wave_max(M);
-            for (uint32_t p = tid & 63; p <= cut.y - cut.x; p += 64) {
-                const uint64_t at = first + paged_slot(p) * a.n_cols;
-                L = fmaf(__builtin_amdgcn_exp2f(a.ml[at * 2] - M), a.ml[at * 2 + 1], L);
-            }
-            L = wave_sum(L);
-        }
-        if ((tid & 63) == 0) {
-            s_h[h] = M - PAGED_P_LOG2;
-            s_h[a.G + h] = L == 0.0f ? 0.0f : 1.0f / L;   // NaN where a page was bad
-        }
-    }
-    __syncthreads();
-    float* const m = a.mass + (static_cast<uint64_t>(s) * c.n_kv + g) * a.mass_stride;
+    float* const mass = a.mass + (static_cast<uint64_t>(s) * c.n_kv + g) * a.mass_stride;
     const float* const sc = a.scores + (static_cast<uint64_t>(s) * c.n_kv + g) * a.G * a.score_stride;
-    // four positions a thread: their loads are in flight together
+    // four positions a thread: their loads are in flight together, and beside those of the sums
     constexpr uint32_t N = PAGED_MASS_POS / 256;
     uint32_t t[N];
     float before[N], sum[N];
@@ -273,9 +250,36 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
     for (uint32_t u = 0; u < N; ++u) {
         const uint32_t i = min(i0 + u * 256 + tid, n_seen - 1);
         t[u] = i < v.sink_end ? i : v.start + (i - v.sink_end);
-        before[u] = m[t[u]];
+        before[u] = mass[t[u]];
         sum[u] = 0.0f;
     }
+    for (uint32_t h = tid >> 6; h < a.G; h += 4) {   // a wavefront per head, its lanes over the parts
+        const uint32_t cg = h / a.n_cols;
+        const uint64_t gh = g * a.n_cg + cg;
+        const uint2 cut_h = a.spans ? a.cut[gh * gridDim.y + s] : make_uint2(0, 0);
+        float M = PAGED_LOWEST, L = 0.0f;
+        if (cut_h.x == cut_h.y) {
+            const float* const ml = a.ml_seq + ((gh * gridDim.y + s) * a.n_cols + h % a.n_cols) * 2;
+            M = ml[0];
+            L = ml[1];
+        } else {
+            const uint64_t first = (gh * 2 * a.spans + 2 * cut_h.x) * a.n_cols + h % a.n_cols;
+            for (uint32_t p = tid & 63; p <= cut_h.y - cut_h.x; p += 64) {
+                const float2 y = *reinterpret_cast<const float2*>(a.ml + (first + paged_slot(p) * a.n_cols) * 2);
+                const float m = fmaxf(M, y.x);
+                L = fmaf(__builtin_amdgcn_exp2f(y.x - m), y.y, L * __builtin_amdgcn_exp2f(M - m));
+                M = m;
+            }
+            const float m = wave_max(M);
+            L = wave_sum(L * __builtin_amdgcn_exp2f(M - m));
+            M = m;
+        }
+        if ((tid & 63) == 0) {
+            s_h[h] = M - PAGED_P_LOG2;
+            s_h[a.G + h] = L == 0.0f ? 0.0f : 1.0f / L;   // NaN where a page was bad
+        }
+    }
+    __syncthreads();
 #pragma unroll 2
     for (uint32_t h = 0; h < a.G; ++h) {
 #pragma unroll
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
     }
 #pragma unroll
     for (uint32_t u = 0; u < N; ++u)
-        if (i0 + u * 256 + tid < n_seen && sum[u] == sum[u]) m[t[u]] = (a.mass_fresh && t[u] == P ? 0.0f : before[u]) + sum[u];
+        if (i0 + u * 256 + tid < n_seen && sum[u] == sum[u]) mass[t[u]] = (a.mass_fresh && t[u] == P ? 0.0f : before[u]) + sum[u];
 }
 
 template <typename KV, int HD>
