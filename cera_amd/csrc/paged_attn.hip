@@ -4,7 +4,9 @@
 #include "paged_chunk.hip.h"
 
 // ---- chunks: the new rows into their pages -----------------------------------------------------------------------------
-// grid = (blocks, sequences); a thread moves four floats of a row's keys and values
+// grid = (blocks, sequences); a thread moves four floats of a row's keys and values.  Bound by memory: 7 us for 2048 rows of 8 kv heads
+// of 128, 25 MB.  Few columns need it not: their workgroups take the new rows from the call's (51.5 us with this launch, 50.2 without,
+// for 16 sequences of 5 drafts).
 template <typename KV, int HD>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __restrict__ kp, KV* __restrict__ vp, const float* __restrict__ k_new,
                                                            const float* __restrict__ v_new, uint64_t kv_stride, const uint32_t* __restrict__ q_first,
@@ -42,7 +44,8 @@ template <typename KV_, int HD> struct PagedMany {
 
 // Groups of columns that are not cut, of all sequences: the longest first, and every second round of the chip the other way round, so
 // that a CU's add up to about the same.  A group's length is its last position's, or the window: item k is found from the number of
-// groups that are at least 32 L long, for which a lane each looks at its sequence.
+// groups that are at least 32 L long, for which a lane each looks at its sequence.  60.4 to 50.0 us for 12 sequences of up to 700 tokens,
+// 63.4 to 57.6 for 8; below 8 sequences the search costs what it saves: 47.0 us without it and 48.9 with it for 6.
 struct PagedItem { uint32_t seq, cg; bool none; };
 __device__ __forceinline__ PagedItem paged_item(const PagedView& c, const PagedOp& a, uint32_t n_seqs, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63, rows = max(1u, a.n_cols / a.G);   // rows of a group
@@ -176,6 +179,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typenam
 // grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 1024 positions of a kv head each.
 // Columns: HD / 4 threads of four values for each of SPLIT shares of a column's parts.  Positions: the scores lie as the attention
 // left them, in the base-2 domain.
+// What bounds it are its launch and two loads in a row: 6.6 us for 16 sequences' 20 rows of 32 heads in about 4 parts each, 4.9 us for two
+// in 64, 10 us with the weights of 32 sequences of up to 8000 positions.
 static constexpr uint32_t PAGED_MASS_POS = 1024;
 // part p of a sequence lies this many slots behind slot 2 (its first workgroup)
 __device__ __forceinline__ uint64_t paged_slot(uint32_t p) { return p == 0 ? 1 : 2 * static_cast<uint64_t>(p); }
@@ -307,7 +312,10 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.scale2 = in.scale * 1.44269504088896340736f;
     a.window = in.window; a.n_sink = in.n_sink;
     const uint64_t cols = static_cast<uint64_t>(a.max_queries) * a.G;
-    const bool many = in.q_first && cols > (HALF ? 32 : 48);
+    // 16 sequences of 4000 positions, few columns' kernel and many columns': half cache, 32 columns 61.8 and 72.6 us, 40 columns 90.6 and 82.0;
+    // f32, 24 columns 147.7 and 141.1, 48 columns 195 and 162.  Few columns of a half cache: 20 columns in one group of 32 take 60.0 us, in two of 16
+    // 67.8, 32 columns 61.8 and 86.1.
+    const bool many = in.q_first && cols > (HALF ? 32 : 16);
     const bool twin = HALF && cols <= 8, two = HALF && cols > 16;
     a.n_cols = many ? 128 : twin ? 8 : two ? 32 : 16;
     a.n_cg = static_cast<uint32_t>((cols + a.n_cols - 1) / a.n_cols);
@@ -358,7 +366,8 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
         if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{});
     }
     if (a.spans || a.mass) {
-        const bool shared = a.spans > 8;   // parts of a column shared out
+        // parts of a column shared out: 13.0 us for one sequence of 8000 positions in 64 parts, 16.2 in one thread's turn; with 6 parts 237 and 215
+        const bool shared = a.spans > 8;
         const uint32_t cols_wg = 256 / (HD / 4 * (shared ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
         const uint32_t mass = a.mass ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;

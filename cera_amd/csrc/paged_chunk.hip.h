@@ -10,7 +10,13 @@
 // which goes into its scores: three products, what is left out is below 2^-21 of one.  Values and weights, whose sum has no room for
 // a power of two a row, become three bfloat16 each, which have f32's range: six products.  All of it takes a quarter of the f32
 // instruction's clocks.
-// What bounds it are the matrix cores, with the softmax between the products in the shadow of the other wavefronts.
+// What bounds it are the matrix cores and the power that they take.  2048 rows at 6000 positions, 32 heads of 128, half cache: 320 to
+// 350 us from card to card, 0.52 to 0.47 PFLOP/s of the operator, twice that of the instruction, where a large library product reaches 1.14;
+// 243 us where all data are zeros and the clock stays up.  The instruction is busy for 57 % of the cycles, the softmax between the
+// products in the shadow of the other wavefronts; a workgroup alone takes 1.1 us a tile, two on a CU 2.2 together.  Keys are in no
+// bank twice.  What did not help: the next scores beside the softmax (spills, twice the time), three buffers, two accumulators of scores.
+// F32 cache: 2.1 us a tile of 64 dims for a lone workgroup, half of it the splitting of values into parts; two buffers of parts, put
+// beside the products, cost the third workgroup a CU its registers: 50 us for 44.
 #pragma once
 #include <type_traits>
 

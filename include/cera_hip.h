@@ -479,7 +479,8 @@ CERA_HIP_API cera_hip_status cera_hip_gemm_dev(cera_hip_ctx*, const cera_hip_dte
  * element p * page_stride (0: one behind the other), both 16-byte aligned; keys are stored rotated.
  * Position t of sequence s is slot t % page_size of page table[s * max_pages + t / page_size].
  * Entries whose positions a call does not use are not read as page numbers and may hold anything.
- * Pages may be shared between sequences as long as no call writes to them.  head_dim 64 or 128;
+ * Pages may be shared between sequences as long as no call writes to them.  What a call reads may not
+ * overlap what it writes, but where a call says so.  head_dim 64 or 128;
  * page_size 16, 32, 64, 128 or 256; at most 65535 sequences and 2^30 positions in a row of the table. */
 typedef struct {
     uint32_t kv_type;    /* CERA_HIP_KV_F32 or CERA_HIP_KV_F16 */
@@ -506,9 +507,17 @@ typedef struct {
  * mass (nullable, decode form): mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
  * g's query heads of the softmax weight of position t.  With k_new and mass_fresh the new position's
  * starts at 0, whatever an eviction or a shortened sequence has left there.
- * Memory: mass and many parts take a workspace of the context (about 4 bytes * n_heads * max_len per
- * sequence for mass).  Results do not depend on other sequences of the call or on earlier calls.
- * Host refusals: n_heads not a multiple of n_kv_heads, scale not finite, pointers not 16-byte (lens,
+ * Keys and values enter as the cache holds them, everything else is f32: products, softmax and sums have f32's
+ * accuracy for both kinds of cache (queries, keys and values below 10^30 and scores that f32 holds).  A row
+ * whose query, or a key that it sees, holds an infinity or NaN gets NaN; of a value that it sees, only the
+ * dim that holds one, which then is not finite either; what a row does not see changes nothing in it.
+ * Long sequences are cut among workgroups and joined, by the lengths of the whole call: the same call
+ * again gives the same bits, another one's may differ by roundings.
+ * Memory: a workspace of the context, grown as needed: parts of cut sequences, at most 70 MB, without which
+ * sequences stay whole, and with mass about 4 bytes * n_heads * max_len per sequence, without which the call
+ * fails (CERA_HIP_ERR_OOM).
+ * Host refusals: n_heads not a multiple of n_kv_heads or above 1024 of them a kv head, scale not finite or above
+ * 10^30, mass with q_first, k_new without v_new, pointers not 16-byte (lens,
  * table, q_first, mass: 4-byte) aligned, strides below a row or no multiple of 4 floats.
  * On the device: a sequence with lens[s] > max_len (0: the table's capacity), a page number outside
  * the pool among the positions it uses, or rows that decrease, end behind n_rows, outnumber
@@ -538,7 +547,8 @@ CERA_HIP_API cera_hip_status cera_hip_paged_attn_dev(cera_hip_ctx*, const cera_h
  * [n_seqs][n_kv_heads][budget]): the former position of each that stays, -1 behind the last.
  * The positions' rank among the kv heads differs, so a cache that has been cut has no position
  * numbers in common with its tokens: a window then counts kept positions.  Pages of the moved
- * positions may not be shared.  n_first + n_recent <= budget, budget >= 1.
+ * positions may not be shared.  n_first + n_recent <= budget, budget >= 1.  Memory: 4 bytes * budget a
+ * kv head and sequence of workspace.
  * A sequence with lens[s] > max_len or a bad page number among its pages is left as it is, with
  * new_lens[s] = lens[s] and kept all -1.  What `shift_kv` does for a run of positions
  * (cera/src/kv_cache.rs:1091-1310) without a choice by weight. */
@@ -564,7 +574,8 @@ CERA_HIP_API cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx*, const cera_
  * uniform and draft are not read.
  * out_tokens[s] = accepted drafts, the next token, then -1.  A row with a NaN or +inf, or with nothing
  * but -inf, ends its sequence with next token -1; so does n_draft[s] > max_draft, with none accepted.
- * A drafted token outside the vocabulary is rejected, and takes nothing away from p. */
+ * A drafted token outside the vocabulary is rejected, and takes nothing away from p.  1 to 64 drafts, a
+ * vocabulary of up to 2^24, at most 65535 sequences.  Memory: 24 bytes of workspace for each 1024 logits. */
 typedef struct {
     uint32_t n_seqs, max_draft, vocab;
     float temperature;        /* 0 to 10^6 */

@@ -177,3 +177,28 @@ def test_refusals(hip):
             hip.verify_draft(A.VerifyDraft(**{**ok, **more}))
         assert e.value.status == status
     hip.verify_draft(A.VerifyDraft(**{**ok, "n_seqs": 0}))
+
+
+def test_the_same_call_many_times(hip):
+    """A sequence's token is drawn by whichever of its workgroups is done last: the same one every time."""
+    r = np.random.default_rng(8)
+    S, D, V = 6, 3, 128256
+    target = (r.standard_normal((S, D + 1, V)) * 2).astype(np.float32)
+    draft = (target[:, :D] + r.standard_normal((S, D, V))).astype(np.float32)
+    tokens = draft.argmax(2).astype(np.int32)
+    bufs = [hip.to_device(x) for x in (target, draft, tokens)]
+    d_u, d_acc, d_out = hip.malloc(S * (D + 1) * 4), hip.malloc(S * 4), hip.malloc(S * (D + 1) * 4)
+    for k in range(40):
+        u = r.random((S, D + 1)).astype(np.float32)
+        hip.upload(d_u, u)
+        hip.verify_draft(A.VerifyDraft(n_seqs=S, max_draft=D, vocab=V, temperature=0.9, target=bufs[0], draft=bufs[1], tokens=bufs[2], uniform=d_u, accepted=d_acc, out_tokens=d_out))
+        got = hip.download(d_out, (S, D + 1), np.int32)
+        if k % 10 == 0:
+            for s in range(S):
+                _, want, near = _ref(target[s], draft[s], tokens[s], D, u[s], 0.9)
+                assert near > 1e-12 and list(got[s]) == list(want), (k, s)
+        for _ in range(5):
+            hip.verify_draft(A.VerifyDraft(n_seqs=S, max_draft=D, vocab=V, temperature=0.9, target=bufs[0], draft=bufs[1], tokens=bufs[2], uniform=d_u, accepted=d_acc, out_tokens=d_out))
+            assert np.array_equal(got, hip.download(d_out, (S, D + 1), np.int32)), k
+    for b in bufs + [d_u, d_acc, d_out]:
+        hip.free(b)
