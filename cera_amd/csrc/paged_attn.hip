@@ -325,7 +325,7 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     const uint32_t wide = c.n_kv_heads * a.n_cg;
     const PagedCut cut = paged_cut(v.max_len, a.max_queries, a.window, a.n_sink, a.tile, wide, c.n_seqs, many, HALF, ctx->n_cu);
     a.spans = cut.spans;
-    a.ordered = many && !a.spans && c.n_seqs >= 8 && c.n_seqs <= 64 && wide * c.n_seqs > ctx->n_cu;
+    a.ordered = many && !a.spans && c.n_seqs >= 8 && c.n_seqs <= 64 && static_cast<uint64_t>(wide) * c.n_seqs > ctx->n_cu && static_cast<uint64_t>(a.n_cg) * c.n_seqs < (1u << 24);
     a.least = cut.least;
     a.score_stride = a.mass ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;
     // scores | results of parts | maxima and sums of parts | of whole sequences | who has a sequence's parts

@@ -34,15 +34,15 @@ struct VdArgs {
     uint32_t* done;    // [seq] workgroups that have their sums
 };
 
-// e^((z - top) / t) for z <= top, as 2^k 2^f with k + f = z c - top c, c = log2 e / t, |f| <= 1/2, and 2^f by its Taylor series to
-// f^11: 6e-15 of the value, and the rounding of z c, 1e-16 of the exponent.  -inf gives 0.
+// e^((z - top) / t) for z <= top, as 2^k 2^f with k + f = (z - top) c, c = log2 e / t, |f| <= 1/2, and 2^f by its Taylor series to
+// f^11: 6e-15 of the value, and the difference's rounding, 2^-53 of the exponent; the largest itself is 1 at every t.  -inf gives 0.
 constexpr double vd_taylor(int n) {   // ln(2)^n / n!
     double x = 1.0;
     for (int i = 1; i <= n; ++i) x *= 0.69314718055994530942 / i;
     return x;
 }
-__device__ __forceinline__ double vd_exp(float z, double c, double top_c) {
-    const double t = fma(static_cast<double>(fmaxf(z, -3.402823466e38f)), c, -top_c), k = __builtin_rint(t), f = t - k;
+__device__ __forceinline__ double vd_exp(float z, double c, double top) {
+    const double t = (static_cast<double>(fmaxf(z, -3.402823466e38f)) - top) * c, k = __builtin_rint(t), f = t - k;
     double p = vd_taylor(11);
     p = fma(p, f, vd_taylor(10));
     p = fma(p, f, vd_taylor(9));
@@ -112,9 +112,8 @@ __global__ __launch_bounds__(VD_THREADS) void verify_rows_kernel(VdArgs a) {
     } else {
         double sum = 0.0;
         if (!bad && top > -__builtin_inff()) {
-            const double top_c = top * a.c;
 #pragma unroll
-            for (uint32_t e = 0; e < VD_PER; ++e) sum += vd_exp(x[e], a.c, top_c);
+            for (uint32_t e = 0; e < VD_PER; ++e) sum += vd_exp(x[e], a.c, top);
             sum = wave_sum_f64(sum);
         }
         if (lane == 0) a.sum[o] = sum;
@@ -152,18 +151,17 @@ __device__ __forceinline__ VdRow vd_whole(const VdArgs& a, uint32_t row, VdPart 
             m = top;
             continue;
         }
-        const double top_c = top * a.c;
-        if (sum > 0.0) sum *= vd_exp(m, a.c, top_c);
+        if (sum > 0.0) sum *= vd_exp(m, a.c, top);
         m = top;
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e)
-            if (c0 + 64 * e + (threadIdx.x & 63) < a.n_chunks && x.t[e] > -__builtin_inff()) sum += x.u[e] * vd_exp(x.t[e], a.c, top_c);
+            if (c0 + 64 * e + (threadIdx.x & 63) < a.n_chunks && x.t[e] > -__builtin_inff()) sum += x.u[e] * vd_exp(x.t[e], a.c, top);
     }
     VdRow r{m, 0.0, !__any(bad) && m > -__builtin_inff()};
     if (r.ok && a.c != 0.0) r.sum = wave_sum_f64(sum);
     return r;
 }
-__device__ __forceinline__ double vd_p(const VdArgs& a, const VdRow& r, float z) { return vd_exp(z, a.c, r.top * a.c) / r.sum; }
+__device__ __forceinline__ double vd_p(const VdArgs& a, const VdRow& r, float z) { return vd_exp(z, a.c, r.top) / r.sum; }
 
 struct VdDecision {
     VdRow p, q;         // of the row that the next token is drawn from
@@ -238,9 +236,9 @@ template <uint32_t N> __device__ __forceinline__ void vd_weights(const VdArgs& a
 #pragma unroll
     for (uint32_t e = 0; e < N; ++e) {
         const uint32_t v = v0 + e * step;
-        w[e] = vd_exp(x[e], a.c, d.p.top * a.c) * inv_p;
+        w[e] = vd_exp(x[e], a.c, d.p.top) * inv_p;
         if (rest) {
-            const double q = y ? vd_exp(u[e], a.c, d.q.top * a.c) * inv_q : v == d.token ? 1.0 : 0.0;
+            const double q = y ? vd_exp(u[e], a.c, d.q.top) * inv_q : v == d.token ? 1.0 : 0.0;
             w[e] = fmax(w[e] - q, 0.0);
         }
         if (v >= a.vocab) w[e] = 0.0;

@@ -125,6 +125,25 @@ def test_random_numbers_at_their_ends(hip, lookup):
         _check(hip, target, draft, tokens, None, uniform, 0.7)
 
 
+@pytest.mark.parametrize("t", [1e-3, 1e-6, 1e-20, 1e-38, 1e-44])
+@pytest.mark.parametrize("lookup", [True, False])
+def test_temperatures_at_which_the_largest_logit_is_all(hip, lookup, t):
+    """Logits a quarter apart around -1000 and 3e37: weights of 1 and 0, whatever (logit / temperature) overflows or loses."""
+    r = np.random.default_rng(2)
+    S, D, V = 4, 3, 3000
+    target = np.stack([[r.permutation(V) * 0.25 - 1000 for _ in range(D + 1)] for _ in range(S)]).astype(np.float32)
+    target[0] = np.where(target[0] > -600, 3e37, -3e37) * (1 + (target[0] + 1000) / 4000)
+    draft = target[:, :D].copy()
+    draft[1, 2] = np.roll(draft[1, 2], 5)
+    draft[2, 0] = np.roll(draft[2, 0], 1)
+    tokens = draft.argmax(2).astype(np.int32)
+    uniform = np.full((S, D + 1), 0.75, np.float32)
+    acc, out = _run(hip, target, None if lookup else draft, tokens, None, uniform, t)
+    best = target.argmax(2)
+    for s, n in enumerate((3, 2, 0, 3)):
+        assert acc[s] == n and list(out[s]) == list(best[s, :n + 1]) + [-1] * (D - n), (s, acc[s], out[s], best[s])
+
+
 @pytest.mark.parametrize("t", [0.0, 1.0])
 @pytest.mark.parametrize("lookup", [True, False])
 def test_masked_tokens_and_bad_rows(hip, lookup, t):
