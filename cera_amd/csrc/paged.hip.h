@@ -47,6 +47,11 @@ __device__ __forceinline__ uint64_t paged_row(const PagedView& v, uint32_t page,
     return page * v.page_stride + g * v.head_stride + static_cast<uint64_t>(t & ((1u << v.page_log2) - 1)) * HD;
 }
 
+// Rows that nothing reads again before the caches have seen much else.
+template <typename T> using PagedRaw = uint32_t __attribute__((ext_vector_type(sizeof(T) / 4)));
+template <typename T> __device__ __forceinline__ T paged_stream(const void* p) { return __builtin_bit_cast(T, __builtin_nontemporal_load(static_cast<const PagedRaw<T>*>(p))); }
+template <typename T> __device__ __forceinline__ void paged_stream(void* p, T x) { __builtin_nontemporal_store(__builtin_bit_cast(PagedRaw<T>, x), static_cast<PagedRaw<T>*>(p)); }
+
 // Infinities and NaN have the largest exponent: the magnitudes' running maximum, as integers, tells whether any is among many.
 typedef unsigned short paged_u2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t paged_most(uint32_t top, uint32_t pair) {   // of halves, both of a pair at once

@@ -9,8 +9,9 @@
 // columns (TWIN) the pair takes columns c and c + 8 of the 16 in one product, else hi and lo have a product each.  q is brought to a
 // largest magnitude of 2^8 by a power of two, the weights to 2^14, so that low halves stay normal.  F32 cache: the f32 matrix
 // instruction, 16 columns.
-// What bounds it is the stream of K and V: 32 sequences of 4000 positions, 8 kv heads of 128, half cache, 104 us for 524 MB, 5.0 TB/s,
-// where a large copy reaches 4.8 and a large sum 4.0; an f32 cache 5.5 TB/s.  Hence: no LDS between memory and the matrix cores (a tile
+// What bounds it is the stream of K and V: 32 sequences of 8000 positions, 8 kv heads of 128, half cache, 162 us for 1.05 GB, 6.5 TB/s,
+// where a large copy reaches 4.8; an f32 cache the same.  Hence: non-temporal loads (187 us without; a cache that the last-level
+// cache still holds costs 5 to 10 % more so, but between two steps of a model come its weights), no LDS between memory and the matrix cores (a tile
 // is read by one wavefront, once), the next tile's keys in flight from behind the scores on and its values from behind the weights on,
 // page numbers by scalar loads, whose wait is not one for the tiles.
 // Eight columns and their low halves in one product cost as much as sixteen without them: 104.2 us, two products 105.0.
@@ -158,7 +159,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
         for (int u = 0; u < SUB; ++u) {
             const uint8_t* const base = reinterpret_cast<const uint8_t*>(kp + at[u]) + k_lane;
 #pragma unroll
-            for (int st = 0; st < KS; ++st) f.k[u][st] = *reinterpret_cast<const std::remove_reference_t<decltype(f.k[u][st])>*>(base + 64 * st);
+            for (int st = 0; st < KS; ++st) f.k[u][st] = paged_stream<std::remove_reference_t<decltype(f.k[u][st])>>(base + 64 * st);
         }
     };
     auto load_v = [&]() __attribute__((always_inline)) {
@@ -169,12 +170,12 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
             for (int p = 0; p < 4; ++p) {
                 if constexpr (!HALF) {
 #pragma unroll
-                    for (int h = 0; h < Tile::VW; ++h) f.v[p][h] = *reinterpret_cast<const float4*>(base + p * HD * 4 + 256 * h);
+                    for (int h = 0; h < Tile::VW; ++h) f.v[p][h] = paged_stream<float4>(base + p * HD * 4 + 256 * h);
                 } else if constexpr (HD == 128) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(base + p * HD * 2);
+                    const uint4 x = paged_stream<uint4>(base + p * HD * 2);
                     f.v[4 * u + p][0] = x.x; f.v[4 * u + p][1] = x.y; f.v[4 * u + p][2] = x.z; f.v[4 * u + p][3] = x.w;
                 } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(base + p * HD * 2);
+                    const uint2 x = paged_stream<uint2>(base + p * HD * 2);
                     f.v[4 * u + p][0] = x.x; f.v[4 * u + p][1] = x.y;
                 }
             }

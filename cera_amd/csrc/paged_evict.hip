@@ -6,9 +6,9 @@
 // written, as long as all rows of a step are read before the step writes.
 //
 // 16 sequences of up to 8192 positions of 8 kv heads of 128, half cache, brought to 4096: the choice takes 14 us, bound by the latency of
-// its passes (a histogram in LDS and a scan each), the move 111 us, bound by memory: about 0.5 GB in and out, 4.8 TB/s, what a large copy
-// reaches.  A workgroup of 1024 threads moves 128 bytes of every row of one kv head's keys or values, two of them a CU (118 us; one a CU
-// 141), the next step's rows on their way while this one's are written.
+// its passes (a histogram in LDS and a scan each), the move 103 us, bound by memory: 0.54 GB in and out, 5.3 TB/s, where a large copy
+// reaches 4.8.  A workgroup of 1024 threads moves 128 bytes of every row of one kv head's keys or values, two of them a CU (one a CU: a fifth
+// more), the next step's rows on their way while this one's are written; non-temporal, 8 us less.
 #include "paged.hip.h"
 
 static constexpr uint32_t EV_THREADS = 1024, EV_BINS = 2048;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(EV_THREADS, 8) void paged_evict_move_kernel(PagedVi
     auto read = [&](Step& x, uint32_t i0) __attribute__((always_inline)) {
 #pragma unroll
         for (uint32_t u = 0; u < EV_UNROLL; ++u)
-            if (x.from[u] != i0 + u * EV_ROWS + r0) x.row[u] = *reinterpret_cast<const uint4*>(at(x.from[u]));
+            if (x.from[u] != i0 + u * EV_ROWS + r0) x.row[u] = paged_stream<uint4>(at(x.from[u]));
     };
     auto write = [&](Step& x, uint32_t i0) __attribute__((always_inline)) {
         // every wavefront has this step's rows in its registers
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(EV_THREADS, 8) void paged_evict_move_kernel(PagedVi
 #pragma unroll
         for (uint32_t u = 0; u < EV_UNROLL; ++u) {
             const uint32_t i = i0 + u * EV_ROWS + r0;
-            if (x.from[u] != i) *reinterpret_cast<uint4*>(at(i)) = x.row[u];
+            if (x.from[u] != i) paged_stream(at(i), x.row[u]);
         }
     };
     Step a, b;
