@@ -14,7 +14,7 @@
 // cache still holds costs 5 to 10 % more so, but between two steps of a model come its weights), no LDS between memory and the matrix cores (a tile
 // is read by one wavefront, once), the next tile's keys in flight from behind the scores on and its values from behind the weights on,
 // page numbers by scalar loads, whose wait is not one for the tiles.
-// Eight columns and their low halves in one product cost as much as sixteen without them: 104.2 us, two products 105.0.
+// Eight columns and their low halves in one product: 167 us for those sequences, with two products 174.
 #pragma once
 #include "paged.hip.h"
 

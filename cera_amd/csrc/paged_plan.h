@@ -137,20 +137,18 @@ inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t windo
     uint64_t most = (static_cast<uint64_t>(max_len) + tile - 1) / tile;
     if (window) most = std::min(most, (static_cast<uint64_t>(window) + max_queries + tile - 1) / tile + 1 + (static_cast<uint64_t>(n_sink) + tile - 1) / tile);
     PagedCut c;
-    // Parts of about equal size, two workgroups a CU (four and eight a CU: 97 and 100 us for 32 sequences of up to 8000 positions where
-    // two take 96, 40 and 40 for 31 behind a window of 1024).  Groups of columns that fill the chip by themselves are not cut, nor are
-    // short sequences: parts cost a launch more, and their results, 64 KB each of a chunk's 128 columns, are written and read again.
-    // Single tokens, half cache, cut and uncut: 13.2 and 15.7 us for one sequence of 900 positions, 17.4 and 15.7 for four, 20.0 and
-    // 29.6 for four of 2400; where there are two workgroups a CU without parts, 72.8 and 67.9 for 64 of 1400, 57.0 and 61.4 for 64 of
-    // up to 2400.  F32 cache, a tile of which takes twice as long: 14.6 and 19.5 us for one of 640, 18.3 and 20.0 for four, 137 and 130
-    // for 64 of 1400, 80 and 86 for 64 of up to 1400.
+    // Parts of about equal size, two workgroups a CU: 84 us for 32 sequences of up to 8000 positions, 90 with one a CU, 92 with three; 31, 32
+    // and 41 behind a window of 1024.  Groups of columns that fill the chip by themselves are not cut, nor are short sequences: parts
+    // cost a launch more, and their results, 64 KB each of a chunk's 128 columns, are written and read again.
+    // Single tokens, half cache, cut and uncut: one sequence of 500 positions 13.5 and 11.7 us, of 900 14.5 and 19.7; four of 640 18.3 and 16.3, of
+    // 900 19.5 and 21.3; where there are two workgroups a CU without parts, 64 of up to 1400 51 and 45, of up to 2400 60 and 73.  F32 cache,
+    // a tile of which takes twice as long: four of up to 500 23.3 and 22.4, of 640 21.9 and 26.7; 64 of 900 87 and 80, of up to 1400 75 and 89.
     // Chunks, up to one workgroup a CU without parts: 38.5 and 49.4 us for 300 tokens at 1000 positions, half cache, 28.8 and 26.6 for
     // 400 tokens; f32 51 and 108, 44.5 and 51.2.  More of them: 74.6 and 49.2 us for six sequences of up to 700 tokens.
     const uint64_t uncut = static_cast<uint64_t>(wide) * n_seqs;
     uint32_t longest;   // that stays whole
     if (chunk) longest = uncut > n_cu ? 1024 : half ? 512 : 256;
     else if (uncut >= 2 * n_cu) longest = half ? 2048 : 1024;
-    else if (n_seqs > 1) longest = half ? 1024 : 512;
     else longest = half ? 640 : 384;
     c.least = 256 / tile;
     c.spans = most * tile <= longest || n_cu < wide || most * n_seqs > 0x7FFFFFFFu ? 0 : 2 * n_cu / wide;

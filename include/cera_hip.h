@@ -516,6 +516,7 @@ typedef struct {
  * Memory: a workspace of the context, grown as needed: parts of cut sequences, at most 70 MB, without which
  * sequences stay whole, and with mass about 4 bytes * n_heads * max_len per sequence, without which the call
  * fails (CERA_HIP_ERR_OOM).
+ * max_len and max_queries also choose how the work is laid out: the nearer to the call's longest, the better.
  * Host refusals: n_heads not a multiple of n_kv_heads or above 1024 of them a kv head, scale not finite or above
  * 10^30, mass with q_first, k_new without v_new, pointers not 16-byte (lens,
  * table, q_first, mass: 4-byte) aligned, strides below a row or no multiple of 4 floats.
