@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typenam
 // grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 1024 positions of a kv head each.
 // Columns: HD / 4 threads of four values for each of SPLIT shares of a column's parts.  Positions: the scores lie as the attention
 // left them, in the base-2 domain.
-// What bounds it are its launch and two loads in a row: 6.6 us for 16 sequences' 20 rows of 32 heads in about 4 parts each, 4.9 us for two
+// What bounds it are its launch and two loads in a row: 6.4 us for 16 sequences' 20 rows of 32 heads in about 4 parts each, 4.7 us for two
 // in 64, 10 us with the weights of 32 sequences of up to 8000 positions.
 static constexpr uint32_t PAGED_MASS_POS = 1024;
 // part p of a sequence lies this many slots behind slot 2 (its first workgroup)

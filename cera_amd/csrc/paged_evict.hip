@@ -6,7 +6,7 @@
 // written, as long as all rows of a step are read before the step writes.
 //
 // 16 sequences of up to 8192 positions of 8 kv heads of 128, half cache, brought to 4096: the choice takes 14 us, bound by the latency of
-// its passes (a histogram in LDS and a scan each), the move 103 us, bound by memory: 0.54 GB in and out, 5.3 TB/s, where a large copy
+// its passes (a histogram in LDS and a scan each), the move 108 us, bound by memory: 0.54 GB in and out, 5.0 TB/s, where a large copy
 // reaches 4.8.  A workgroup of 1024 threads moves 128 bytes of every row of one kv head's keys or values, two of them a CU (one a CU: a fifth
 // more), the next step's rows on their way while this one's are written; non-temporal, 8 us less.
 #include "paged.hip.h"
