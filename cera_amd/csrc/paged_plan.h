@@ -140,15 +140,21 @@ inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t windo
     // Parts of about equal size, two workgroups a CU: 84 us for 32 sequences of up to 8000 positions, 90 with one a CU, 92 with three; 31, 32
     // and 41 behind a window of 1024.  Groups of columns that fill the chip by themselves are not cut, nor are short sequences: parts
     // cost a launch more, and their results, 64 KB each of a chunk's 128 columns, are written and read again.
-    // Single tokens, half cache, cut and uncut: one sequence of 500 positions 13.5 and 11.7 us, of 900 14.5 and 19.7; four of 640 18.3 and 16.3, of
-    // 900 19.5 and 21.3; where there are two workgroups a CU without parts, 64 of up to 1400 51 and 45, of up to 2400 60 and 73.  F32 cache,
-    // a tile of which takes twice as long: four of up to 500 23.3 and 22.4, of 640 21.9 and 26.7; 64 of 900 87 and 80, of up to 1400 75 and 89.
-    // Chunks, up to one workgroup a CU without parts: 38.5 and 49.4 us for 300 tokens at 1000 positions, half cache, 28.8 and 26.6 for
-    // 400 tokens; f32 51 and 108, 44.5 and 51.2.  More of them: 74.6 and 49.2 us for six sequences of up to 700 tokens.
+    // Single tokens, half cache, cut and uncut, by the number of workgroups without parts: 8 of them, 500 positions 13.5 and 11.7 us, 900
+    // 14.5 and 19.7; 32, 640 18.3 and 16.3, 900 19.5 and 21.3; 192, 1056 behind a window 32.8 and 26.4, 1400 35.0 and 30.9, of up to 1400 26.2 and 27.7, of up
+    // to 2000 29.8 and 36.1; 256, 2000 52 and 45, of up to 3000 46 and 52.  F32 cache, a tile of which takes twice as long: 32, of up to 500 23.3
+    // and 22.4, 640 21.9 and 26.7; 128, 640 32.7 and 28.6, 900 36.1 and 40.1; 256, 900 52 and 44; 512, of up to 1400 75 and 89.
+    // Chunks, up to one workgroup a CU without parts: 300 tokens at 1000 positions 38.5 and 49.4 us, 400 tokens 28.8 and 26.6; f32 51 and 108,
+    // 44.5 and 51.2.  More of them: six sequences of up to 700 tokens 74.6 and 49.2; 384, 30 tokens at 1500 144 and 106, at up to 1500 107
+    // and 76, 60 at up to 4000 144 and 166, f32 30 at up to 1500 142 and 167; 512, 100 tokens at 2000 193 and 129, at up to 2000 140 and 96,
+    // f32 334 and 268, 203 and 215; 640, f32 300 at 3000 531 and 441, at up to 3000 280 and 318.
     const uint64_t uncut = static_cast<uint64_t>(wide) * n_seqs;
     uint32_t longest;   // that stays whole
-    if (chunk) longest = uncut > n_cu ? 1024 : half ? 512 : 256;
-    else if (uncut >= 2 * n_cu) longest = half ? 2048 : 1024;
+    if (chunk && uncut >= 2 * n_cu) longest = half ? 4096 : 2048;
+    else if (chunk && 2 * uncut >= 3 * n_cu) longest = half ? 2048 : 1024;
+    else if (chunk) longest = uncut > n_cu ? 1024 : half ? 512 : 256;
+    else if (uncut >= n_cu) longest = half ? 2048 : 1024;
+    else if (8 * uncut >= 3 * n_cu) longest = half ? 1280 : 640;
     else longest = half ? 640 : 384;
     c.least = 256 / tile;
     c.spans = most * tile <= longest || n_cu < wide || most * n_seqs > 0x7FFFFFFFu ? 0 : 2 * n_cu / wide;
