@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(PagedView c, typenam
 // grid = (workgroups, sequences): those of the columns first, then (a.mass) those of 1024 positions of a kv head each.
 // Columns: HD / 4 threads of four values for each of SPLIT shares of a column's parts.  Positions: the scores lie as the attention
 // left them, in the base-2 domain.
-// What bounds it are its launch and two loads in a row: 6.6 us for 16 sequences' 20 rows of 32 heads in about 4 parts each, 4.9 us for two
+// What bounds it are its launch and two loads in a row: 4.8 us for 16 sequences' 5 rows of 32 heads in about 4 parts each, 4.9 us for two
 // in 64, 10 us with the weights of 32 sequences of up to 8000 positions.
 static constexpr uint32_t PAGED_MASS_POS = 1024;
 // part p of a sequence lies this many slots behind slot 2 (its first workgroup)
@@ -313,9 +313,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.scale2 = in.scale * 1.44269504088896340736f;
     a.window = in.window; a.n_sink = in.n_sink;
     const uint64_t cols = static_cast<uint64_t>(a.max_queries) * a.G;
-    // 16 sequences of 4000 positions, few columns' kernel and many columns': half cache, 32 columns 61.8 and 72.6 us, 40 columns 90.6 and 82.0;
-    // f32, 24 columns 147.7 and 141.1, 48 columns 195 and 162.  Few columns of a half cache: 20 columns in one group of 32 take 60.0 us, in two of 16
-    // 67.8, 32 columns 61.8 and 86.1.
+    // 16 sequences of 4000 positions, few columns' kernel and many columns': half cache, 32 columns 67 and 81 us, 40 columns 103 and 85;
+    // f32, 16 columns 96 and 142, 20 columns 149 and 142.  Few columns of a half cache: 20 columns in one group of 32 take 64 us, in two of 16
+    // 85, 32 columns 67 and 96.
     const bool many = in.q_first && cols > (HALF ? 32 : 16);
     const bool twin = HALF && cols <= 8, two = HALF && cols > 16;
     a.n_cols = many ? 128 : twin ? 8 : two ? 32 : 16;
@@ -367,8 +367,10 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
         if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{});
     }
     if (a.spans || a.mass) {
-        // parts of a column shared out: 13.0 us for one sequence of 8000 positions in 64 parts, 16.2 in one thread's turn; with 6 parts 237 and 215
-        const bool shared = a.spans > 8;
+        // A column's parts shared out among eight: 15.8 us for one sequence of 8000 positions in 64 parts, 17.6 in one thread's turn; 1000 rows
+        // in 6 parts 236 and 218.  Of more columns than make two thousand workgroups few have so many parts: 81 and 72 us for 48 sequences
+        // of 5 rows, 74 and 64 for 16 of 20.
+        const bool shared = a.spans > 8 && static_cast<uint64_t>(wide) * a.n_cols * c.n_seqs <= 2048;
         const uint32_t cols_wg = 256 / (HD / 4 * (shared ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
         const uint32_t mass = a.mass ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;

@@ -144,15 +144,15 @@ inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t windo
     // 14.5 and 19.7; 32, 640 18.3 and 16.3, 900 19.5 and 21.3; 192, 1056 behind a window 32.8 and 26.4, 1400 35.0 and 30.9, of up to 1400 26.2 and 27.7, of up
     // to 2000 29.8 and 36.1; 256, 2000 52 and 45, of up to 3000 46 and 52.  F32 cache, a tile of which takes twice as long: 32, of up to 500 23.3
     // and 22.4, 640 21.9 and 26.7; 128, 640 32.7 and 28.6, 900 36.1 and 40.1; 256, 900 52 and 44; 512, of up to 1400 75 and 89.
-    // Chunks, up to one workgroup a CU without parts: 300 tokens at 1000 positions 38.5 and 49.4 us, 400 tokens 28.8 and 26.6; f32 51 and 108,
-    // 44.5 and 51.2.  More of them: six sequences of up to 700 tokens 74.6 and 49.2; 384, 30 tokens at 1500 144 and 106, at up to 1500 107
-    // and 76, 60 at up to 4000 144 and 166, f32 30 at up to 1500 142 and 167; 512, 100 tokens at 2000 193 and 129, at up to 2000 140 and 96,
-    // f32 334 and 268, 203 and 215; 640, f32 300 at 3000 531 and 441, at up to 3000 280 and 318.
+    // Chunks: up to one workgroup a CU without parts, 300 tokens at 1000 positions 38 and 51 us, 400 tokens 30 and 28, f32 52 and 110, 44 and 50;
+    // up to two, two sequences of 600 tokens 52 and 44, 30 tokens at up to 3000 for 48 of them 114 and 135, f32 two of up to 600 57 and 74; two
+    // and more, 100 tokens at 2000 149 and 127, at up to 2000 95 and 96, 300 at up to 3000 150 and 145, 100 at up to 4000 149 and 169, f32 six of 700
+    // 224 and 183, 100 at up to 2000 158 and 216.
     const uint64_t uncut = static_cast<uint64_t>(wide) * n_seqs;
     uint32_t longest;   // that stays whole
-    if (chunk && uncut >= 2 * n_cu) longest = half ? 4096 : 2048;
-    else if (chunk && 2 * uncut >= 3 * n_cu) longest = half ? 2048 : 1024;
-    else if (chunk) longest = uncut > n_cu ? 1024 : half ? 512 : 256;
+    if (chunk && uncut >= 2 * n_cu) longest = half ? 3200 : 1024;
+    else if (chunk && uncut > n_cu) longest = half ? 1024 : 512;
+    else if (chunk) longest = half ? 512 : 256;
     else if (uncut >= n_cu) longest = half ? 2048 : 1024;
     else if (8 * uncut >= 3 * n_cu) longest = half ? 1280 : 640;
     else longest = half ? 640 : 384;
