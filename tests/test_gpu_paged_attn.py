@@ -261,6 +261,30 @@ def test_infinities_reach_only_the_rows_that_see_them(hip, f16, heads, n_kv, hd,
 
 
 @pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("heads,n_kv,n_seqs,window,sinks", [(32, 8, 12, 0, 0), (32, 8, 12, 40, 3), (24, 8, 15, 0, 0), (8, 8, 64, 0, 0), (16, 4, 70, 0, 0), (72, 4, 9, 100, 0)])
+def test_chunks_of_many_sequences(hip, f16, heads, n_kv, n_seqs, window, sinks):
+    """Uncut groups of columns of ragged sequences, longest first (up to 64 of them) or in order, with empty and faulty ones among them."""
+    print("many", f16, heads, n_kv, n_seqs, window, sinks, flush=True)
+    r = np.random.default_rng(n_seqs)
+    lens = [int(x) for x in r.integers(1, 260, n_seqs)]
+    counts = [int(min(n, c)) for n, c in zip(lens, r.integers(0, 130 if n_seqs < 20 else 40, n_seqs))]
+    lens[2], counts[2] = 0, 0
+    counts[4], lens[4] = 33, 259
+    counts[6] = min(lens[6], 5)
+    pool = P.Pool(hip, lens, n_kv, 64, f16, 32, seed=3)
+    rows = P.Rows(pool, sum(counts), heads, seed=4, new=True)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.uint32)
+    bad = np.array(lens, np.uint32)
+    bad[6] = pool.cols * pool.page + 1            # longer than its row of the table
+    hip.paged_attn(pool.kv(lens=pool.dev(bad)), rows.op(q_first=pool.dev(first), max_queries=max(counts), window=window, n_sink=sinks))
+    _new_rows(pool, rows, lens, counts)
+    got = rows.result()
+    _check(pool, rows, counts, window, sinks, got, skip=(6,))
+    assert np.isnan(got[first[6]:first[7]]).all()
+    pool.close()
+
+
+@pytest.mark.parametrize("f16", [True, False])
 @pytest.mark.parametrize("heads,n_kv,hd", [(2, 2, 64), (8, 1, 64), (4, 1, 128), (40, 1, 128)])
 @pytest.mark.parametrize("window", [0, 2])
 def test_new_values_that_are_not_finite(hip, f16, heads, n_kv, hd, window):
