@@ -237,7 +237,7 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
             }
         }
         if (!mine) return;
-        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        const float inv = 1.0f / L;
         o.x *= inv; o.y *= inv; o.z *= inv; o.w *= inv;
         *reinterpret_cast<float4*>(a.out + (r.first + static_cast<uint64_t>(col / a.G)) * a.out_stride + (g * a.G + col % a.G) * HD + 4 * x) = o;
         return;

@@ -108,6 +108,17 @@ template <bool TWIN> __device__ __forceinline__ void paged_pair(float x, float y
     }
 }
 
+// A query's values as halves, high ones rounded away from 0: low ones then have the other sign, or are 0, and a key that is infinite
+// gives inf - inf or inf * 0, which is NaN, whatever the signs.  A NaN stays one in the low half.
+typedef _Float16 paged_h2 __attribute__((ext_vector_type(2)));
+typedef float paged_f2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t paged_near(float x, float y) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(paged_f2{x, y}, paged_h2)); }   // to the nearest even
+__device__ __forceinline__ void paged_query(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const float a = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) + ~PAGED_HIGH) & PAGED_HIGH), b = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, y) + ~PAGED_HIGH) & PAGED_HIGH);
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    lo = paged_near(x - a, y - b);
+}
+
 template <int NC, int HD> struct PagedShared {
     __attribute__((aligned(16))) float o[4][NC][HD + 4];
     float m[4][NC], l[4][NC];
@@ -263,12 +274,14 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
             int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
             up = min(up, 100);
             mul[b] = ldexpf(a.scale2, -up);
-            const uint32_t mask = low ? PAGED_HIGH : 0u;
 #pragma unroll
             for (int st = 0; st < KS; ++st) {
                 uint32_t d[4], n[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) paged_pair<TWIN>(ldexpf(x[st][2 * e], up), ldexpf(x[st][2 * e + 1], up), mask, d[e], n[e]);
+                for (int e = 0; e < 4; ++e) {
+                    paged_query(ldexpf(x[st][2 * e], up), ldexpf(x[st][2 * e + 1], up), d[e], n[e]);
+                    if (low) d[e] = n[e];
+                }
                 if constexpr (AWAY) {
                     if (w == static_cast<uint32_t>(b)) {
                         q_away[(2 * (b * KS + st)) * 64] = make_uint4(d[0], d[1], d[2], d[3]);
@@ -286,12 +299,16 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
     }
 
     if constexpr (AWAY) lds_barrier();
-    float m[CB], l[CB];
+    // An infinity or NaN in a query or in a key that it sees makes their score not finite.  +inf and NaN reach the sum by themselves;
+    // -inf, whose weight would be 0, cannot come from a half cache (paged_query); over an f32 cache it shows in the smallest score that a
+    // lane has seen: 129 us for 128 of two sequences of up to 60000.
+    float m[CB], l[CB], least[HALF ? 1 : CB];
     paged_f4 o[CB][NO];
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
         m[b] = PAGED_LOWEST;
         l[b] = 0.0f;
+        if constexpr (!HALF) least[b] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NO; ++i) o[b][i] = paged_f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -350,8 +367,13 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
 #pragma unroll
                 for (int p = 0; p < NS; ++p) {
                     const uint32_t t = t0 + 16 * (p >> 2) + 4 * lg + (p & 3);
-                    if (!(t < sink[b] || (t >= start[b] && t <= P[b]))) x[b][p] = -__builtin_inff();
+                    const bool sees = t < sink[b] || (t >= start[b] && t <= P[b]);
+                    if constexpr (!HALF) least[b] = fminf(least[b], sees ? x[b][p] : 0.0f);
+                    if (!sees) x[b][p] = -__builtin_inff();
                 }
+            } else if constexpr (!HALF) {
+#pragma unroll
+                for (int p = 0; p < NS; ++p) least[b] = fminf(least[b], x[b][p]);
             }
             if (MASS) {
                 if (!low && col[b] <= c_last) {
@@ -485,8 +507,9 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
     // ---- the four wavefronts joined
 #pragma unroll
     for (int b = 0; b < CB; ++b) {
-        l[b] = paged_xor_sum(l[b]);
+        if constexpr (!HALF) l[b] = least[b] == -__builtin_inff() ? __builtin_nanf("") : l[b];
         if (!ok) l[b] = __builtin_nanf("");
+        l[b] = paged_xor_sum(l[b]);
         const uint32_t lcol = b * CW + (TWIN ? lc & 7 : lc);
         if (lg == 0 && !low) {
             sh.m[w][lcol] = m[b];
@@ -524,7 +547,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
             x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         if (alone) {
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            const float inv = 1.0f / L;   // a row sees itself
             *reinterpret_cast<float4*>(a.out + (r.first + static_cast<uint64_t>(cc / a.G)) * a.out_stride + (g * a.G + cc % a.G) * HD + d) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
             if (MASS && d == 0) *reinterpret_cast<float2*>(a.ml_seq + ((static_cast<uint64_t>(gx) * a.n_rows + s) * NC + lcol) * 2) = make_float2(M, L);
         } else {

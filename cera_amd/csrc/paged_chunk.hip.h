@@ -203,10 +203,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             const float y[8] = {f[2 * st].x * by, f[2 * st].y * by, f[2 * st].z * by, f[2 * st].w * by, f[2 * st + 1].x * by, f[2 * st + 1].y * by, f[2 * st + 1].z * by, f[2 * st + 1].w * by};
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e], y[2 * e + 1]));
-                lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16)));
-            }
+            for (int e = 0; e < 4; ++e) paged_query(y[2 * e], y[2 * e + 1], hi[e], lo[e]);
             qh[st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             ql[st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
@@ -395,7 +392,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
     if (col > c_last) return;
     const uint64_t item = (static_cast<uint64_t>(g * a.n_cg + cg) * 2 * a.spans + slot) * a.n_cols + 32 * w + lc;
     float* const to = alone ? a.out + (r.first + static_cast<uint64_t>(qi)) * a.out_stride + h * HD : a.acc + item * HD;
-    const float inv = !alone ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = !alone ? 1.0f : 1.0f / l;   // a row sees itself
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
