@@ -282,18 +282,21 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
         }
         if ((tid & 63) == 0) {
             s_h[h] = M - PAGED_P_LOG2;
-            s_h[a.G + h] = L == 0.0f ? 0.0f : 1.0f / L;   // NaN where a page was bad
+            s_h[a.G + h] = L > 0.0f ? 1.0f / L : 0.0f;   // a head that is no number, or has met a bad page, adds nothing
         }
     }
     __syncthreads();
 #pragma unroll 2
     for (uint32_t h = 0; h < a.G; ++h) {
 #pragma unroll
-        for (uint32_t u = 0; u < N; ++u) sum[u] = fmaf(__builtin_amdgcn_exp2f(sc[h * a.score_stride + t[u]] - s_h[h]), s_h[a.G + h], sum[u]);
+        for (uint32_t u = 0; u < N; ++u)   // an exponent is 14 at most, but for NaN: 0 times any number is 0
+            sum[u] = fmaf(__builtin_amdgcn_exp2f(fminf(sc[h * a.score_stride + t[u]] - s_h[h], 100.0f)), s_h[a.G + h], sum[u]);
     }
 #pragma unroll
-    for (uint32_t u = 0; u < N; ++u)
-        if (i0 + u * 256 + tid < n_seen && sum[u] == sum[u]) mass[t[u]] = (a.mass_fresh && t[u] == P ? 0.0f : before[u]) + sum[u];
+    for (uint32_t u = 0; u < N; ++u) {
+        const bool fresh = a.mass_fresh && t[u] == P;
+        if (i0 + u * 256 + tid < n_seen && (fresh || sum[u] != 0.0f)) mass[t[u]] = (fresh ? 0.0f : before[u]) + sum[u];
+    }
 }
 
 template <typename KV, int HD>

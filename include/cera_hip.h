@@ -506,7 +506,8 @@ typedef struct {
  * be in pages of their own sequence only.
  * mass (nullable, decode form): mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
  * g's query heads of the softmax weight of position t.  With k_new and mass_fresh the new position's
- * starts at 0, whatever an eviction or a shortened sequence has left there.
+ * starts at 0, whatever an eviction or a shortened sequence has left there.  A query head whose row is NaN
+ * (a query or key that is not finite, a bad page) adds nothing; the kv head's others add theirs.
  * Keys and values enter as the cache holds them, everything else is f32: products, softmax and sums have f32's
  * accuracy for both kinds of cache (queries, keys and values below 10^30 and scores that f32 holds).  A row
  * whose query, or a key that it sees, holds an infinity or NaN gets NaN; of a value that it sees, only the
@@ -523,8 +524,8 @@ typedef struct {
  * On the device: a sequence with lens[s] > max_len (0: the table's capacity), a page number outside
  * the pool among the positions it uses, or rows that decrease, end behind n_rows, outnumber
  * max_queries or lens[s], gets NaN in its rows of out, and neither its pages nor its mass change
- * unless all of its lengths and rows are in order (with a bad page, rows and weights that live
- * in good pages may have been written). */
+ * unless all of its lengths and rows are in order (with a bad page, rows that live in good pages may have
+ * been written, and of the weights mass_fresh's 0). */
 typedef struct {
     const float *q, *k_new, *v_new; /* rows of n_heads / n_kv_heads / n_kv_heads * head_dim floats */
     float* out;
