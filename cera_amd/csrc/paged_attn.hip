@@ -27,6 +27,14 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedView c, KV* __re
         KvOps<KV>::st4(vp + dst, c4, *reinterpret_cast<const float4*>(v_new + src + 4 * c4));
     }
 }
+// their weights to 0, in a launch of its own: as arguments of the other it cost each call 0.4 us
+__global__ __launch_bounds__(256) void paged_fresh_kernel(PagedView c, float* __restrict__ mass, uint64_t mass_stride, const uint32_t* __restrict__ q_first, uint32_t n_rows, uint32_t max_queries) {
+    const uint32_t s = blockIdx.y;
+    const PagedRows r = paged_rows(q_first, c.lens, s, n_rows, max_queries, c.max_len);
+    if (r.bad) return;
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < static_cast<uint64_t>(r.n) * c.n_kv; i += gridDim.x * 256ull)
+        mass[(static_cast<uint64_t>(s) * c.n_kv + i / r.n) * mass_stride + (r.len - r.n + i % r.n)] = 0.0f;
+}
 
 // ---- attention ------------------------------------------------------------------------------------------------------
 template <typename KV_, int HD, int CB, bool TWIN, bool MASS> struct PagedFew {
@@ -304,10 +312,12 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     constexpr bool HALF = sizeof(KV) == 2;
     const PagedView v = paged_view(c, in.max_len);
     PagedOp a{};
-    a.q = in.q; a.out = in.out; a.mass = in.mass; a.q_first = in.q_first;
+    a.q = in.q; a.out = in.out; a.q_first = in.q_first;
     a.q_stride = in.q_stride ? in.q_stride : static_cast<uint64_t>(in.n_heads) * HD;
     a.out_stride = in.out_stride ? in.out_stride : static_cast<uint64_t>(in.n_heads) * HD;
     a.kv_stride = in.kv_stride ? in.kv_stride : static_cast<uint64_t>(c.n_kv_heads) * HD;
+    a.mass = in.mass;
+    const bool weights = in.mass && !in.q_first;
     a.mass_stride = in.mass_stride;
     a.mass_fresh = in.k_new && in.mass_fresh;
     a.n_rows = in.n_rows;
@@ -331,9 +341,9 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.spans = cut.spans;
     a.ordered = many && !a.spans && c.n_seqs >= 8 && c.n_seqs <= 64 && static_cast<uint64_t>(wide) * c.n_seqs > ctx->n_cu && static_cast<uint64_t>(a.n_cg) * c.n_seqs < (1u << 24);
     a.least = cut.least;
-    a.score_stride = a.mass ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;
+    a.score_stride = weights ? (static_cast<uint64_t>(v.max_len) + 31) / 32 * 32 : 0;
     // scores | results of parts | maxima and sums of parts | of whole sequences | who has a sequence's parts
-    const uint64_t scores = a.score_stride * c.n_seqs * in.n_heads, seqs = static_cast<uint64_t>(wide) * c.n_seqs, ml_seq = a.mass ? seqs * a.n_cols * 2 : 0;
+    const uint64_t scores = a.score_stride * c.n_seqs * in.n_heads, seqs = static_cast<uint64_t>(wide) * c.n_seqs, ml_seq = weights ? seqs * a.n_cols * 2 : 0;
     auto parts = [&] { return static_cast<uint64_t>(wide) * 2 * a.spans * a.n_cols; };
     auto bytes = [&] { return 4 * (scores + parts() * (HD + 2) + ml_seq + (a.spans ? 2 * seqs : 0)); };
     void* ws = nullptr;
@@ -348,9 +358,11 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     a.ml_seq = a.ml + parts() * 2;
     a.cut = reinterpret_cast<uint2*>(a.ml_seq + ml_seq);
     if (in.k_new && many) {
-        const uint64_t items = static_cast<uint64_t>(a.max_queries) * c.n_kv_heads * (HD / 4);
-        hipLaunchKernelGGL((paged_append_kernel<KV, HD>), dim3(static_cast<uint32_t>(std::min<uint64_t>((items + 255) / 256, 1024)), c.n_seqs), dim3(256), 0, ctx->stream, v,
-                           static_cast<KV*>(c.k), static_cast<KV*>(c.v), in.k_new, in.v_new, a.kv_stride, a.q_first, a.n_rows, a.max_queries);
+        auto blocks = [&](uint64_t items) { return dim3(static_cast<uint32_t>(std::min<uint64_t>((items + 255) / 256, 1024)), c.n_seqs); };
+        const uint64_t rows = static_cast<uint64_t>(a.max_queries) * c.n_kv_heads;
+        hipLaunchKernelGGL((paged_append_kernel<KV, HD>), blocks(rows * (HD / 4)), dim3(256), 0, ctx->stream, v, static_cast<KV*>(c.k), static_cast<KV*>(c.v), in.k_new, in.v_new, a.kv_stride,
+                           a.q_first, a.n_rows, a.max_queries);
+        if (in.mass) hipLaunchKernelGGL(paged_fresh_kernel, blocks(rows), dim3(256), 0, ctx->stream, v, in.mass, in.mass_stride, a.q_first, a.n_rows, a.max_queries);
     } else {
         a.k_new = in.k_new;
         a.v_new = in.v_new;
@@ -363,20 +375,20 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     if (many) {
         launch(PagedMany<KV, HD>{});
     } else if constexpr (HALF) {
-        if (twin) { if (a.mass) launch(PagedFew<KV, HD, 1, true, true>{}); else launch(PagedFew<KV, HD, 1, true, false>{}); }
-        else if (two) { if (a.mass) launch(PagedFew<KV, HD, 2, false, true>{}); else launch(PagedFew<KV, HD, 2, false, false>{}); }
-        else { if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{}); }
+        if (twin) { if (weights) launch(PagedFew<KV, HD, 1, true, true>{}); else launch(PagedFew<KV, HD, 1, true, false>{}); }
+        else if (two) { if (weights) launch(PagedFew<KV, HD, 2, false, true>{}); else launch(PagedFew<KV, HD, 2, false, false>{}); }
+        else { if (weights) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{}); }
     } else {
-        if (a.mass) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{});
+        if (weights) launch(PagedFew<KV, HD, 1, false, true>{}); else launch(PagedFew<KV, HD, 1, false, false>{});
     }
-    if (a.spans || a.mass) {
+    if (a.spans || weights) {
         // A column's parts shared out among eight: 15.8 us for one sequence of 8000 positions in 64 parts, 17.6 in one thread's turn; 1000 rows
         // in 6 parts 236 and 218.  Of more columns than make two thousand workgroups few have so many parts: 81 and 72 us for 48 sequences
         // of 5 rows, 74 and 64 for 16 of 20.
         const bool shared = a.spans > 8 && static_cast<uint64_t>(wide) * a.n_cols * c.n_seqs <= 2048;
         const uint32_t cols_wg = 256 / (HD / 4 * (shared ? 8 : 1)), merge = a.spans ? wide * ((a.n_cols + cols_wg - 1) / cols_wg) : 0;
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
-        const uint32_t mass = a.mass ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;
+        const uint32_t mass = weights ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;
         const dim3 blocks(merge + mass * c.n_kv_heads, c.n_seqs);
         if (shared) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
         else hipLaunchKernelGGL((paged_finish_kernel<HD, 1>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);

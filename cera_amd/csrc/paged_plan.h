@@ -61,7 +61,7 @@ inline PagedCheck paged_check_attn(const cera_hip_paged_kv* c, const cera_hip_pa
         return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: a stride is below a row, or no multiple of 4");
     if (!paged_aligned(a->q, 16) || !paged_aligned(a->out, 16) || !paged_aligned(a->k_new, 16) || !paged_aligned(a->v_new, 16) || !paged_aligned(a->q_first, 4) || !paged_aligned(a->mass, 4))
         return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: q, k_new, v_new and out are 16-byte aligned, q_first and mass 4-byte");
-    if (a->mass && a->q_first) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: mass goes with one row a sequence");
+    if (a->mass && a->q_first && !(a->mass_fresh && a->k_new)) return paged_no(CERA_HIP_ERR_ARGUMENT, "paged attention: mass with q_first only sets the new positions' to 0 (mass_fresh, k_new)");
     if (a->mass && (a->mass_stride < paged_max_len(*c, a->max_len) || a->mass_stride > (1ull << 40))) return paged_no(CERA_HIP_ERR_SHAPE, "paged attention: mass_stride is below the longest sequence");
     return {CERA_HIP_OK, nullptr};
 }

@@ -504,9 +504,11 @@ typedef struct {
  * k_new / v_new (both or neither): the rows' own keys and values, [n_rows][n_kv_heads * head_dim]
  * f32, which are written into the pages first (narrowed to half to the nearest even) and so have to
  * be in pages of their own sequence only.
- * mass (nullable, decode form): mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
+ * mass (nullable), in the decode form: mass[(s * n_kv_heads + g) * mass_stride + t] += the sum over kv head
  * g's query heads of the softmax weight of position t.  With k_new and mass_fresh the new position's
- * starts at 0, whatever an eviction or a shortened sequence has left there.  A query head whose row is NaN
+ * starts at 0, whatever an eviction or a shortened sequence has left there.  With q_first no weights are added:
+ * mass then needs mass_fresh and k_new, and only the new positions' are set, to 0, which a chunk has to do
+ * whose positions an eviction or a shortened sequence had before.  A query head whose row is NaN
  * (a query or key that is not finite, a bad page) adds nothing; the kv head's others add theirs.
  * Keys and values enter as the cache holds them, everything else is f32: products, softmax and sums have f32's
  * accuracy for both kinds of cache (queries, keys and values below 10^30 and scores that f32 holds).  A row
@@ -519,7 +521,7 @@ typedef struct {
  * fails (CERA_HIP_ERR_OOM).
  * max_len and max_queries also choose how the work is laid out: the nearer to the call's longest, the better.
  * Host refusals: n_heads not a multiple of n_kv_heads or above 1024 of them a kv head, scale not finite or above
- * 10^30, mass with q_first, k_new without v_new, pointers not 16-byte (lens,
+ * 10^30, mass with q_first but for mass_fresh and k_new, k_new without v_new, pointers not 16-byte (lens,
  * table, q_first, mass: 4-byte) aligned, strides below a row or no multiple of 4 floats.
  * On the device: a sequence with lens[s] > max_len (0: the table's capacity), a page number outside
  * the pool among the positions it uses, or rows that decrease, end behind n_rows, outnumber
@@ -547,6 +549,8 @@ CERA_HIP_API cera_hip_status cera_hip_paged_attn_dev(cera_hip_ctx*, const cera_h
  * mass move down in place to positions 0 .. budget - 1.  new_lens[s] = min(lens[s], budget), which
  * the caller uses as lens from then on (it may not be the array lens itself); kept (nullable,
  * [n_seqs][n_kv_heads][budget]): the former position of each that stays, -1 behind the last.
+ * Behind the budget, rows and mass stay as they were: what takes these positions next sets their mass
+ * to 0 (mass_fresh).
  * The positions' rank among the kv heads differs, so a cache that has been cut has no position
  * numbers in common with its tokens: a window then counts kept positions.  Pages of the moved
  * positions may not be shared.  n_first + n_recent <= budget, budget >= 1.  Memory: 4 bytes * budget a
