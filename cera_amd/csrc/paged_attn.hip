@@ -194,7 +194,7 @@ static constexpr uint32_t PAGED_MASS_POS = 1024;
 // part p of a sequence lies this many slots behind slot 2 (its first workgroup)
 __device__ __forceinline__ uint64_t paged_slot(uint32_t p) { return p == 0 ? 1 : 2 * static_cast<uint64_t>(p); }
 template <int HD, int SPLIT>
-__global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, PagedOp a, uint32_t merge_blocks, uint32_t mass_blocks) {
+__global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, PagedOp a, uint32_t merge_blocks, uint32_t mass_blocks, float p_log2) {
     constexpr uint32_t COLS = 256 / (HD / 4 * SPLIT);
     __shared__ __attribute__((aligned(16))) float4 s_o[SPLIT > 1 ? 256 : 1];
     __shared__ float s_m[SPLIT > 1 ? 256 : 1], s_l[SPLIT > 1 ? 256 : 1];
@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
             M = m;
         }
         if ((tid & 63) == 0) {
-            s_h[h] = M - PAGED_P_LOG2;
+            s_h[h] = M - p_log2;
             s_h[a.G + h] = L > 0.0f ? 1.0f / L : 0.0f;   // a head that is no number, or has met a bad page, adds nothing
         }
     }
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(256, 8) void paged_finish_kernel(PagedView c, Paged
 #pragma unroll 2
     for (uint32_t h = 0; h < a.G; ++h) {
 #pragma unroll
-        for (uint32_t u = 0; u < N; ++u)   // an exponent is 14 at most, but for NaN: 0 times any number is 0
+        for (uint32_t u = 0; u < N; ++u)   // an exponent is p_log2 at most, but for NaN: 0 times any number is 0
             sum[u] = fmaf(__builtin_amdgcn_exp2f(fminf(sc[h * a.score_stride + t[u]] - s_h[h], 100.0f)), s_h[a.G + h], sum[u]);
     }
 #pragma unroll
@@ -390,8 +390,8 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
         const uint64_t most = a.window ? std::min<uint64_t>(v.max_len, static_cast<uint64_t>(a.window) + a.n_sink) : v.max_len;
         const uint32_t mass = weights ? static_cast<uint32_t>((most + PAGED_MASS_POS - 1) / PAGED_MASS_POS) : 0;
         const dim3 blocks(merge + mass * c.n_kv_heads, c.n_seqs);
-        if (shared) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
-        else hipLaunchKernelGGL((paged_finish_kernel<HD, 1>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass);
+        if (shared) hipLaunchKernelGGL((paged_finish_kernel<HD, 8>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass, paged_p_log2<KV>);
+        else hipLaunchKernelGGL((paged_finish_kernel<HD, 1>), blocks, dim3(256), a.G * 8, ctx->stream, v, a, merge, mass, paged_p_log2<KV>);
     }
     HIP_TRY(ctx, hipGetLastError());
     return CERA_HIP_OK;

@@ -19,7 +19,9 @@
 #include "paged.hip.h"
 
 #define PAGED_LOWEST (-3.402823466e38f)   // a running maximum before any score: finite, so that -inf has weight 0
-#define PAGED_P_LOG2 14.0f                // weights are held times 2^14
+// Weights are held times 2^14 for a half cache, whose values are below 2^16; for an f32 cache times 2^-4, so that 2^30 of them on values of
+// 10^30 stay in f32's range.
+template <typename KV> constexpr float paged_p_log2 = sizeof(KV) == 2 ? 14.0f : -4.0f;
 
 typedef float paged_f4 __attribute__((ext_vector_type(4)));
 typedef _Float16 paged_h8 __attribute__((ext_vector_type(8)));
@@ -392,7 +394,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
 #pragma unroll
                 for (int i = 0; i < NO; ++i) o[b][i] *= f0;
             }
-            const float base = m[b] - PAGED_P_LOG2;
+            const float base = m[b] - paged_p_log2<KV>;
 #pragma unroll
             for (int p = 0; p < NS; ++p) {
                 x[b][p] = __builtin_amdgcn_exp2f(x[b][p] - base);

@@ -325,7 +325,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
         for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
         if (__any(top > m)) {
             m = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-            const float b = m == PAGED_LOWEST ? base : fmaf(m, mul, -PAGED_P_LOG2), f0 = __builtin_amdgcn_exp2f(base - b);
+            const float b = m == PAGED_LOWEST ? base : fmaf(m, mul, -paged_p_log2<KV>), f0 = __builtin_amdgcn_exp2f(base - b);
             base = b;
             l *= f0;
 #pragma unroll
@@ -398,5 +398,5 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
 #pragma unroll
         for (int e = 0; e < 4; ++e)
             *reinterpret_cast<float4*>(to + 32 * i + 8 * e + 4 * half) = make_float4(o[i][4 * e] * inv, o[i][4 * e + 1] * inv, o[i][4 * e + 2] * inv, o[i][4 * e + 3] * inv);
-    if (!alone && half == 0) *reinterpret_cast<float2*>(a.ml + item * 2) = make_float2(base + PAGED_P_LOG2, l);
+    if (!alone && half == 0) *reinterpret_cast<float2*>(a.ml + item * 2) = make_float2(base + paged_p_log2<KV>, l);
 }
