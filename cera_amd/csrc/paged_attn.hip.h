@@ -500,7 +500,7 @@ __device__ __forceinline__ void paged_attn_part(PagedShared<(TWIN ? 8 : 16) * CB
 
     // ---- the new rows into their pages, by the workgroup that has the last one's tile
     if (a.k_new && cg == (r.n * a.G - 1) / NC && j_end == tiles.n) {
-        if (a.q_first && a.mass)   // a chunk's new positions start at no weight
+        if (!MASS && a.q_first && a.mass)   // a chunk's new positions start at no weight
             for (uint32_t i = tid; i < r.n; i += 256) a.mass[(static_cast<uint64_t>(s) * c.n_kv + g) * a.mass_stride + new0 + i] = 0.0f;
         for (uint32_t i = tid; i < r.n * (HD / 2); i += 256) {
             const uint32_t t = new0 + i / (HD / 2), part = i % (HD / 2), c4 = part % (HD / 4);

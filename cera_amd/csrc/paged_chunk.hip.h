@@ -196,8 +196,11 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
         int up = top > 0.0f && top < __builtin_inff() ? 9 - __builtin_amdgcn_frexp_expf(top) : 0;   // |q| 2^up < 2^9
         up = min(up, 100);
         q_up = up;
-        mul = PAIRS ? fabsf(a.scale2) : ldexpf(fabsf(a.scale2), -up);
-        const float by = ldexpf(a.scale2 < 0.0f ? -1.0f : 1.0f, up);   // the sign too, so that the largest product is the largest score
+        // The scale's fraction goes into the query: a score is then its product times a power of two, exactly, whatever its size, and with the
+        // sign the largest product is the largest score.
+        const int e = __builtin_amdgcn_frexp_expf(a.scale2);
+        mul = ldexpf(1.0f, min(PAIRS ? e : e - up, 127));
+        const float by = ldexpf(__builtin_amdgcn_frexp_mantf(a.scale2), up);
 #pragma unroll
         for (int st = 0; st < KS; ++st) {
             const float y[8] = {f[2 * st].x * by, f[2 * st].y * by, f[2 * st].z * by, f[2 * st].w * by, f[2 * st + 1].x * by, f[2 * st + 1].y * by, f[2 * st + 1].z * by, f[2 * st + 1].w * by};
@@ -208,12 +211,15 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             ql[st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
-    float m = PAGED_LOWEST, base = -1e30f, l = 0.0f;   // largest product; its score less the weights' exponent; sum of weights
+    float m = PAGED_LOWEST, base = PAGED_LOWEST, l = 0.0f;   // largest product; its score less the weights' exponent; sum of weights
     paged_f16v o[ND];
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
+
+    // From 2^24 on a score has no room for the weights' factor: rounded, it would give weights that a half does not hold.
+    auto base_of = [&](float top) { return PAIRS || fabsf(top) < 16777216.0f ? top - paged_p_log2<KV> : top; };
 
     // where a lane reads: keys by row lc, pieces 2 st + half; values by rows 4 half + (lane & 15) / 4, dims 16 (lane / 16 & 1) + 4 (lane & 3)
     const uint32_t v_row = 4 * half + (lane >> 2 & 3), v_piece = 2 * (lane >> 4 & 1) + (lane >> 1 & 1), v_byte = 8 * (lane & 1);
@@ -325,7 +331,7 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
         for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
         if (__any(top > m)) {
             m = fmaxf(m, fmaxf(top, __shfl_xor(top, 32)));
-            const float b = m == PAGED_LOWEST ? base : fmaf(m, mul, -paged_p_log2<KV>), f0 = __builtin_amdgcn_exp2f(base - b);
+            const float b = m == PAGED_LOWEST ? base : base_of(m * mul), f0 = __builtin_amdgcn_exp2f(base - b);   // from nothing seen: 0
             base = b;
             l *= f0;
 #pragma unroll

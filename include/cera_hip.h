@@ -512,7 +512,7 @@ typedef struct {
  * (a query or key that is not finite, a bad page) adds nothing; the kv head's others add theirs.
  * Keys and values enter as the cache holds them, everything else is f32: products, softmax and sums have f32's
  * accuracy for both kinds of cache (queries, keys and values below 10^30, values below 10^-30 to within
- * 10^-36, and scores that f32 holds).  A row
+ * 10^-36, and scores that f32 holds; beyond 10^7, where f32 itself tells few weights apart, to within 2^-10 over a half cache).  A row
  * whose query, or a key that it sees, holds an infinity or NaN gets NaN; of a value that it sees, only the
  * dim that holds one, which then is not finite either; what a row does not see changes nothing in it.
  * Long sequences are cut among workgroups and joined, by the lengths of the whole call: the same call
