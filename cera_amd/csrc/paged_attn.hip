@@ -347,7 +347,10 @@ static cera_hip_status paged_attn_launch(cera_hip_ctx* ctx, const cera_hip_paged
     auto parts = [&] { return static_cast<uint64_t>(wide) * 2 * a.spans * a.n_cols; };
     auto bytes = [&] { return 4 * (scores + parts() * (HD + 2) + ml_seq + (a.spans ? 2 * seqs : 0)); };
     void* ws = nullptr;
-    if (a.spans) {
+    // A workspace that has to grow takes half as much again, if there is room: it waits for all that is queued, and the scores of a longest
+    // sequence that rises from call to call would need it anew every 32 positions.
+    if (ctx->scratch[15] && bytes() > ctx->scratch_bytes[15]) CERA_TRY(cera_scratch_if_room(ctx, 15, bytes() + bytes() / 2, &ws));
+    if (a.spans && !ws) {
         CERA_TRY(cera_scratch_if_room(ctx, 15, bytes(), &ws));
         if (!ws) a.spans = 0;
     }

@@ -517,9 +517,10 @@ typedef struct {
  * dim that holds one, which then is not finite either; what a row does not see changes nothing in it.
  * Long sequences are cut among workgroups and joined, by the lengths of the whole call: the same call
  * again gives the same bits, another one's may differ by roundings.
- * Memory: a workspace of the context, grown as needed: parts of cut sequences, at most 70 MB, without which
- * sequences stay whole, and with mass about 4 bytes * n_heads * max_len per sequence, without which the call
- * fails (CERA_HIP_ERR_OOM).
+ * Memory: a workspace of the context: parts of cut sequences, at most 70 MB, without which sequences stay
+ * whole, and with mass about 4 bytes * n_heads * max_len per sequence, without which the call fails
+ * (CERA_HIP_ERR_OOM).  Where it has to grow, the call waits for what is queued, and takes half as much again if there
+ * is room, so that a max_len that rises from call to call costs that a few times only.
  * max_len and max_queries also choose how the work is laid out: the nearer to the call's longest, the better.
  * Host refusals: n_heads not a multiple of n_kv_heads or above 1024 of them a kv head, scale not finite or above
  * 10^30, mass with q_first but for mass_fresh and k_new, k_new without v_new, pointers not 16-byte (lens,
