@@ -78,7 +78,7 @@ inline PagedCheck paged_check_evict(const cera_hip_paged_kv* c, const cera_hip_p
 }
 
 inline PagedCheck verify_check(const cera_hip_verify_draft* d) {
-    if (!d || !d->target || !d->tokens || !d->uniform || !d->accepted || !d->out_tokens) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: a pointer is null");
+    if (!d || !d->target || !d->tokens || (!d->uniform && d->temperature != 0) || !d->accepted || !d->out_tokens) return paged_no(CERA_HIP_ERR_ARGUMENT, "verify_draft: a pointer is null");
     if (d->vocab == 0 || d->vocab > (1u << 24)) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: a vocabulary of 1 to 2^24 tokens");
     if (d->max_draft == 0 || d->max_draft > 64) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: 1 to 64 drafted tokens");
     if (d->n_seqs > 65535) return paged_no(CERA_HIP_ERR_SHAPE, "verify_draft: at most 65535 sequences");

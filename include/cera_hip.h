@@ -579,7 +579,7 @@ CERA_HIP_API cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx*, const cera_
  * running sum in the order of the vocabulary exceeds uniform[max_draft] times its total.  All in
  * 64 bits; logits may be -inf (such a token is never drawn).  temperature 0: a token is accepted if it
  * is the row's largest logit (the lowest index of equals), and the next token is that of row j;
- * uniform and draft are not read.
+ * uniform and draft are not read and may be null.
  * out_tokens[s] = accepted drafts, the next token, then -1.  A row with a NaN or +inf, or with nothing
  * but -inf, ends its sequence with next token -1; so does n_draft[s] > max_draft, with none accepted.
  * A drafted token outside the vocabulary is rejected, and takes nothing away from p.  1 to 64 drafts, a

@@ -30,5 +30,11 @@ int main() {
     no(CERA_HIP_ERR_ARGUMENT, "mass of a chunk that is not to be set", [](auto& x) { x.mass_fresh = 0; });
     no(CERA_HIP_ERR_ARGUMENT, "mass of a chunk without new rows", [](auto& x) { x.k_new = x.v_new = nullptr; });
     no(CERA_HIP_ERR_SHAPE, "mass stride of a chunk", [](auto& x) { x.mass_stride = 31; });
+    // at temperature 0 no random number and no draft's distribution is read
+    cera_hip_verify_draft d{};
+    d.n_seqs = 1; d.max_draft = 2; d.vocab = 10; d.target = mem; d.tokens = table; d.accepted = lens; d.out_tokens = table;
+    expect(!verify_check(&d).msg, "no random numbers at temperature 0");
+    d.temperature = 1e-30f;
+    expect(verify_check(&d).msg && verify_check(&d).st == CERA_HIP_ERR_ARGUMENT, "no random numbers at a temperature");
     return failures != 0;
 }
