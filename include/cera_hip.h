@@ -529,7 +529,8 @@ typedef struct {
  * the pool among the positions it uses, or rows that decrease, end behind n_rows, outnumber
  * max_queries or lens[s], gets NaN in its rows of out, and neither its pages nor its mass change
  * unless all of its lengths and rows are in order (with a bad page, rows that live in good pages may have
- * been written, and of the weights mass_fresh's 0). */
+ * been written, and of the weights mass_fresh's 0).  Where q_first goes back and rises again, rows that two sequences
+ * count as theirs have the result of either. */
 typedef struct {
     const float *q, *k_new, *v_new; /* rows of n_heads / n_kv_heads / n_kv_heads * head_dim floats */
     float* out;
@@ -582,7 +583,8 @@ CERA_HIP_API cera_hip_status cera_hip_paged_evict_dev(cera_hip_ctx*, const cera_
  * uniform and draft are not read and may be null.
  * out_tokens[s] = accepted drafts, the next token, then -1.  A row with a NaN or +inf, or with nothing
  * but -inf, ends its sequence with next token -1; so does n_draft[s] > max_draft, with none accepted.
- * A drafted token outside the vocabulary is rejected, and takes nothing away from p.  1 to 64 drafts, a
+ * A drafted token outside the vocabulary is rejected; the next is then drawn from max(p_j - q_j, 0) of the draft's
+ * row, or, looked up, from p_j.  1 to 64 drafts, a
  * vocabulary of up to 2^24, at most 65535 sequences.  Memory: 24 bytes of workspace for each 1024 logits. */
 typedef struct {
     uint32_t n_seqs, max_draft, vocab;
