@@ -7,9 +7,9 @@
 // Half cache: loads go straight into LDS, the next tile's while this one is multiplied, one barrier a tile; the exchange is made on the
 // way in, by what a lane loads.
 // F32 cache: keys become pairs of halves on their way into LDS, brought to a largest magnitude below 2^15 by a power of two of each row,
-// which goes into its scores: three products, what is left out is below 2^-21 of one.  Values and weights, whose sum has no room for
-// a power of two a row, become three bfloat16 each, which have f32's range: six products.  All of it takes a quarter of the f32
-// instruction's clocks.
+// which goes into its scores: three products.  A query and a key are then off by 2^-23 at most, and the product of their low halves, which
+// is left out, is below 2^-22.  Values and weights, whose sum has no room for a power of two a row, become three bfloat16 each, which
+// have f32's range: six products.  All of it takes a quarter of the f32 instruction's clocks.
 // What bounds it are the matrix cores and the power that they take.  2048 rows at 6000 positions, 32 heads of 128, half cache: 320 to
 // 350 us from card to card, 0.52 to 0.47 PFLOP/s of the operator, twice that of the instruction, where a large library product reaches 1.14;
 // 243 us where all data are zeros and the clock stays up.  The instruction is busy for 57 % of the cycles, the softmax between the
@@ -153,8 +153,8 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
                 uint32_t hi[2], lo[2], v[2][3];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    hi[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e], y[2 * e + 1]));
-                    lo[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16)));
+                    hi[e] = paged_near(y[2 * e], y[2 * e + 1]);
+                    lo[e] = paged_near(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16));
                 }
                 paged_thirds(fv[i].x, fv[i].y, v[0]);
                 paged_thirds(fv[i].z, fv[i].w, v[1]);
@@ -206,7 +206,14 @@ __device__ __forceinline__ void paged_chunk_part(PagedChunkShared<KV, HD>& sh, c
             const float y[8] = {f[2 * st].x * by, f[2 * st].y * by, f[2 * st].z * by, f[2 * st].w * by, f[2 * st + 1].x * by, f[2 * st + 1].y * by, f[2 * st + 1].z * by, f[2 * st + 1].w * by};
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) paged_query(y[2 * e], y[2 * e + 1], hi[e], lo[e]);
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (PAIRS) {   // a key that is infinite is NaN in its second half
+                    hi[e] = paged_near(y[2 * e], y[2 * e + 1]);
+                    lo[e] = paged_near(y[2 * e] - h2f(hi[e] & 0xFFFF), y[2 * e + 1] - h2f(hi[e] >> 16));
+                } else {
+                    paged_query(y[2 * e], y[2 * e + 1], hi[e], lo[e]);
+                }
+            }
             qh[st] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
             ql[st] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }

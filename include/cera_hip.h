@@ -510,9 +510,11 @@ typedef struct {
  * mass then needs mass_fresh and k_new, and only the new positions' are set, to 0, which a chunk has to do
  * whose positions an eviction or a shortened sequence had before.  A query head whose row is NaN
  * (a query or key that is not finite, a bad page) adds nothing; the kv head's others add theirs.
- * Keys and values enter as the cache holds them, everything else is f32: products, softmax and sums have f32's
- * accuracy for both kinds of cache (queries, keys and values below 10^30, values below 10^-30 to within
- * 10^-36, and scores that f32 holds; beyond 10^7, where f32 itself tells few weights apart, to within 2^-10 over a half cache).  A row
+ * Keys and values enter as the cache holds them, but that with q_first and more than 16 columns (max_queries times
+ * the query heads of a kv head) an f32 cache's keys are held to 23 bits; queries and weights are held to 22 bits at
+ * least, sums to f32's 24.  So results have f32's accuracy for both kinds of cache (queries, keys and values below
+ * 10^30, values below 10^-30 to within 10^-36, and scores that f32 holds; beyond 10^7, where f32 itself tells few
+ * weights apart, to within 2^-10 over a half cache).  A row
  * whose query, or a key that it sees, holds an infinity or NaN gets NaN; of a value that it sees, only the
  * dim that holds one, which then is not finite either; what a row does not see changes nothing in it.
  * Long sequences are cut among workgroups and joined, by the lengths of the whole call: the same call

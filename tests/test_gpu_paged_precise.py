@@ -29,3 +29,31 @@ def test_every_part_counts(hip, f16, hd, heads, n_kv, counts, lens):
     print("largest error over its bound", worst, flush=True)
     assert worst <= 1
     pool.close()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts", [[1], [3], [40]])
+def test_keys_of_an_f32_cache_to_their_last_bits(hip, hd, counts):
+    """Two scores of 1024 and 1024.5 and a little, in powers of two, that f32 holds: the key is off by half a step of its second half, 2^-23,
+    so the score by 2^-13, and the weight's share of the two, p = 0.59, by ln 2 p (1 - p) times that; the rest, as in paged_precise, is
+    below 2^-18."""
+    n, m = 60, counts[0]
+    scale = np.float32(np.log(2))
+    assert np.float32(scale * np.float32(1.44269504088896340736)) == 1
+    k, v = np.zeros((n, 1, hd), np.float32), np.zeros((n, 1, hd), np.float32)
+    k[:, 0, 3] = -4
+    k[7, 0, 3], k[12, 0, 3] = 1 + 2.0 ** -11 + 3 * 2.0 ** -23, 1
+    v[7] = 1
+    pool = P.Pool(hip, [n], 1, hd, False, 32, seed=3, k=[k], v=[v])
+    rows = P.Rows(pool, m, 4, seed=5)
+    rows.q[:] = 0
+    rows.q[..., 3] = 1024
+    hip.upload(rows.d_q, rows.q)
+    more = {} if m == 1 else dict(q_first=pool.dev(np.array([0, m], np.uint32)))
+    hip.paged_attn(pool.kv(), rows.op(scale=float(scale), **more))
+    w = 2.0 ** (0.5 + 3 * 2.0 ** -13)
+    p = w / (1 + w)
+    err = np.abs(rows.result() - p).max()
+    print("share off by", err, flush=True)
+    assert err <= np.log(2) * p * (1 - p) * 2.0 ** -13 + 2.0 ** -18
+    pool.close()
