@@ -4,7 +4,7 @@
 #include "paged_chunk.hip.h"
 
 // ---- chunks: the new rows into their pages -----------------------------------------------------------------------------
-// grid = (blocks, sequences); a thread moves four floats of a row's keys and values.  Bound by memory: 7 us for 2048 rows of 8 kv heads
+// grid = (blocks, sequences); a thread moves four floats of a row's keys and values.  Bound by memory: 6 to 7 us for 2048 rows of 8 kv heads
 // of 128, 25 MB.  Few columns need it not: their workgroups take the new rows from the call's (51.5 us with this launch, 50.2 without,
 // for 16 sequences of 5 drafts).
 template <typename KV, int HD>
@@ -54,7 +54,7 @@ template <typename KV_, int HD> struct PagedMany {
 // that a CU's add up to about the same.  A group's length is its last position's, or the window: item k is found from the number of
 // groups that are at least 32 L long, for which a lane each looks at its sequence.  128 to 101 us for 24 sequences with 100
 // tokens each at up to 2000 positions, 60 to 50 for 12 of up to 700 tokens, 273 to 203 for 8 with 300 each at 3000; below 8 sequences the search costs
-// what it saves: 6 of up to 700 tokens 46.7 without it and 49.7 with it, of 700 91.0 and 88.4.
+// what it saves: 6 of up to 700 tokens 46.7 without it and 49.7 with it, of 700 91.0 and 88.4.  Above 64, more than a wavefront's lanes, the table's order.
 struct PagedItem { uint32_t seq, cg; bool none; };
 __device__ __forceinline__ PagedItem paged_item(const PagedView& c, const PagedOp& a, uint32_t n_seqs, uint32_t k) {
     const uint32_t lane = threadIdx.x & 63, rows = max(1u, a.n_cols / a.G);   // rows of a group

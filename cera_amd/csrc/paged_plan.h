@@ -148,6 +148,7 @@ inline PagedCut paged_cut(uint32_t max_len, uint32_t max_queries, uint32_t windo
     // up to two, two sequences of 600 tokens 52 and 44, 30 tokens at up to 3000 for 48 of them 114 and 135, f32 two of up to 600 57 and 74; two
     // and more, 100 tokens at 2000 149 and 127, at up to 2000 95 and 96, 300 at up to 3000 150 and 145, 100 at up to 4000 149 and 169, f32 six of 700
     // 224 and 183, 100 at up to 2000 158 and 216.
+    // Workgroups without parts are counted as if every sequence had max_queries rows, above and here: chunks of few rows beside the longest count for more.
     const uint64_t uncut = static_cast<uint64_t>(wide) * n_seqs;
     uint32_t longest;   // that stays whole
     if (chunk && uncut >= 2 * n_cu) longest = half ? 3200 : 1024;
